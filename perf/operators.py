@@ -268,7 +268,7 @@ def _distill(x, ids, values, weights, temperature, normalize):
     out, v = x.dtype, x.shape[1]
     d, _, s, empty, bad = _statistics(x.float(), temperature)
     log_s = torch.log(s)
-    named = (ids >= 0) & (ids < v) & (values > -math.inf)
+    named = (ids >= 0) & (ids < v) & (values != -math.inf)
     at = ids.clamp(0, v - 1).long()
     values = torch.where(named, values, -math.inf)
     if normalize:
@@ -278,7 +278,7 @@ def _distill(x, ids, values, weights, temperature, normalize):
     p = torch.where(named, torch.exp(values), 0.0)
     scale = weights[:, None] * temperature
     idle = empty | (scale == 0) | ~named.any(1, keepdim=True)
-    part = torch.where(p > 0, p * (values - (d.gather(1, at) - log_s)), 0.0)
+    part = torch.where(p == 0, 0.0, p * (values - (d.gather(1, at) - log_s)))
     loss = temperature * scale * part.sum(1, keepdim=True)
     dx = p.sum(1, keepdim=True) * torch.exp(d) / s
     dx.scatter_add_(1, at, -p)
