@@ -39,6 +39,11 @@ pub const LG_DTYPE_F32: lg_dtype = 1;
 pub const LG_DTYPE_F16: lg_dtype = 2;
 pub const LG_DTYPE_BF16: lg_dtype = 3;
 
+pub type lg_head_dtype = u32;
+pub const LG_DTYPE_E4M3: lg_head_dtype = 16;
+pub const LG_DTYPE_E8M0: lg_head_dtype = 17;
+pub const LG_DTYPE_I32: lg_head_dtype = 18;
+
 #[repr(C)]
 #[derive(Clone, Copy)]
 pub struct lg_view {
@@ -208,6 +213,33 @@ extern "C" {
                                     out: *mut u8, out_len: u64) -> lg_core_error;
     pub fn lg_backend_upload_into(ctx: *mut lg_ctx, stream: *mut c_void, bytes: *const u8,
                                   len: u64, t: *const lg_tensor) -> lg_core_error;
+
+    // A language model's head: 8-bit block products, log probabilities, distillation.
+    pub fn lg_backend_quantize_blocks(ctx: *mut lg_ctx, stream: *mut c_void, x: *const lg_tensor,
+                                      q: *const lg_tensor, scales: *const lg_tensor)
+        -> lg_core_error;
+    pub fn lg_backend_gemm_blocks(ctx: *mut lg_ctx, stream: *mut c_void, a: *const lg_tensor,
+                                  a_scales: *const lg_tensor, b: *const lg_tensor,
+                                  b_scales: *const lg_tensor, c: *const lg_tensor, alpha: f32,
+                                  beta: f32) -> lg_core_error;
+    pub fn lg_backend_token_logprobs(ctx: *mut lg_ctx, stream: *mut c_void,
+                                     logits: *const lg_tensor, tokens: *const lg_tensor,
+                                     temperature: f32, logprobs: *const lg_tensor,
+                                     entropy: *const lg_tensor, stats: *const lg_tensor,
+                                     top_logprobs: *const lg_tensor, top_ids: *const lg_tensor)
+        -> lg_core_error;
+    pub fn lg_backend_token_logprobs_backward(ctx: *mut lg_ctx, stream: *mut c_void,
+                                              logits: *const lg_tensor, tokens: *const lg_tensor,
+                                              temperature: f32, stats: *const lg_tensor,
+                                              entropy: *const lg_tensor,
+                                              dlogprobs: *const lg_tensor,
+                                              dentropy: *const lg_tensor,
+                                              dlogits: *const lg_tensor) -> lg_core_error;
+    pub fn lg_backend_distill_grad(ctx: *mut lg_ctx, stream: *mut c_void,
+                                   logits: *const lg_tensor, teacher_ids: *const lg_tensor,
+                                   teacher_logprobs: *const lg_tensor, weights: *const lg_tensor,
+                                   temperature: f32, normalize: i32, losses: *const lg_tensor,
+                                   dlogits: *const lg_tensor) -> lg_core_error;
 
     // The wire format and its device-buffer ends.
     pub fn lg_wire_write_header(dtype: u32, shape: *const u64, rank: u32, out: *mut u8,

@@ -351,6 +351,95 @@ lg_core_error lg_backend_upload_into(lg_ctx* ctx, void* stream, const uint8_t* b
                                      uint64_t len, const lg_tensor* t);
 
 /* ---------------------------------------------------------------------------------------
+ * A language model's head: no counterpart in the reference
+ *
+ * What a pipeline's last stage computes around its products: 8-bit quantization with a scale for
+ * each block of 128, products of such operands, what logits say about given tokens, and the loss
+ * against a teacher. The conventions are the Backend ops': every check runs before `ctx` is used
+ * (first failure wins: a tag that is neither lg_dtype nor lg_head_dtype LG_CORE_WIRE; null
+ * operands, ranks, extents and scalars LG_CORE_SHAPE; element types LG_CORE_DTYPE; layouts
+ * LG_CORE_UNSUPPORTED_LAYOUT; an operand reaching past its storage LG_CORE_SHAPE; an output
+ * whose bytes intersect another operand's LG_CORE_ALIAS), on any error nothing is launched or
+ * written, and calls enqueue on `stream` (NULL = context stream) and return before the device
+ * finishes. Matrices have rows of unit stride at any pitch of at least their length and at any
+ * offset (a window of a larger matrix); vectors have unit stride. Extents are below 2^31 - 256.
+ * Rows that are split over workgroups, and distill_grad, use the context's shared scratch: under
+ * stream capture see "Split scratch" above. Results do not depend on the order in which
+ * workgroups run.
+ * ------------------------------------------------------------------------------------- */
+
+/* Element types of these operators beside lg_dtype's; no wire tags. */
+typedef enum lg_head_dtype {
+    LG_DTYPE_E4M3 = 16, /* OCP FP8: four exponent bits, three of significand, no infinity */
+    LG_DTYPE_E8M0 = 17, /* a scale: 2^(byte - 127), 255 = NaN */
+    LG_DTYPE_I32 = 18
+} lg_head_dtype;
+
+/* q, scales = x with a scale for each block of 128 columns and one row or 128 rows. x [R, C] is
+ * F32, F16 or BF16, or the transpose_matrix view of such a matrix; q [R, C] E4M3; scales F32 or
+ * E8M0 of shape [R, ceil(C/128)] (a scale for each row) or [ceil(R/128), ceil(C/128)].
+ * With A the largest magnitude of a block, at least 2^-100: F32 scales are A/448 and q is
+ * x * (448/A) (each operation rounded to f32), E8M0 scales the smallest power of two s with
+ * A <= 448 s and q is x/s; then rounded to E4M3, to nearest, ties to even. A block that holds an
+ * infinity or a NaN has a NaN scale and NaN elements. */
+lg_core_error lg_backend_quantize_blocks(lg_ctx* ctx, void* stream, const lg_tensor* x,
+                                         const lg_tensor* q, const lg_tensor* scales);
+
+/* c = alpha * A.B + beta * c, where A and B are what (a, a_scales) and (b, b_scales) stand for:
+ * a [M, K] E4M3, b [K, N] the transpose_matrix view of a row-major E4M3 matrix [N, K], scales as
+ * quantize_blocks writes them for a and for that [N, K] matrix (both F32 or both E8M0), c [M, N]
+ * F32, F16 or BF16. A block's 128 products are summed by the matrix cores, the blocks in f32 in a
+ * fixed order; alpha * sum and beta * c add in f32 and round once to c's type. beta = 0 does not
+ * read c; alpha = 0 reads neither a nor b. */
+lg_core_error lg_backend_gemm_blocks(lg_ctx* ctx, void* stream, const lg_tensor* a,
+                                     const lg_tensor* a_scales, const lg_tensor* b,
+                                     const lg_tensor* b_scales, const lg_tensor* c, float alpha,
+                                     float beta);
+
+/* Of each row of logits [R, V] (F32, F16 or BF16), with p = softmax(logits / temperature):
+ * logprobs[r] = log p of tokens[r] (I32; both may be NULL; 0 for a token outside [0, V));
+ * entropy[r] = -sum p log p (may be NULL); stats [R, 2] = (largest logit, log of the sum of
+ * exp((logit - largest) / temperature)), which the gradient needs (may be NULL); and the k
+ * likeliest alternatives, top_logprobs and top_ids [R, k], k <= 128 (both may be NULL), larger
+ * logits first and lower ids first among equal ones. Outputs are F32, ids I32.
+ * A logit of -inf has no probability and is no alternative; places that no alternative takes
+ * have id -1 and log probability -inf. A row of -inf alone: log probability -inf, entropy 0,
+ * stats (-inf, -inf). A row with a NaN or +inf: NaN, and ids -1. Sums are f32 over eight elements
+ * and f64 above. */
+lg_core_error lg_backend_token_logprobs(lg_ctx* ctx, void* stream, const lg_tensor* logits,
+                                        const lg_tensor* tokens, float temperature,
+                                        const lg_tensor* logprobs, const lg_tensor* entropy,
+                                        const lg_tensor* stats, const lg_tensor* top_logprobs,
+                                        const lg_tensor* top_ids);
+
+/* dlogits = the gradient of sum(dlogprobs * logprobs) + sum(dentropy * entropy) with respect to
+ * logits, from token_logprobs' stats and (with dentropy) entropy; dentropy may be NULL. dlogits
+ * has logits' type and may be logits itself. A row of -inf alone gets zeros, a row with a NaN or
+ * +inf NaN; a token outside [0, V) has no gradient. */
+lg_core_error lg_backend_token_logprobs_backward(lg_ctx* ctx, void* stream, const lg_tensor* logits,
+                                                 const lg_tensor* tokens, float temperature,
+                                                 const lg_tensor* stats, const lg_tensor* entropy,
+                                                 const lg_tensor* dlogprobs,
+                                                 const lg_tensor* dentropy,
+                                                 const lg_tensor* dlogits);
+
+/* Distillation from a teacher's likeliest alternatives: with q = softmax(logits / temperature)
+ * and p_i from teacher_logprobs [R, k] (F32, log probabilities at that temperature) of
+ * teacher_ids [R, k] (I32), k <= 128 - the softmax of the row's list if `normalize` is not 0,
+ * their exponentials otherwise -
+ *   losses[r] = weights[r] * temperature^2 * sum_i p_i (log p_i - log q_i)
+ * and dlogits = the gradient of sum(losses). weights (F32, may be NULL: ones). dlogits has
+ * logits' type, may be logits itself, and may be NULL: losses only. An id outside [0, V) or a log
+ * probability of -inf is no entry; an id given twice counts as both. A row without weight (it is
+ * not read), without entries, or of -inf alone has loss 0 and gradient 0; any other row with a
+ * NaN or +inf NaN. token_logprobs' top outputs are such lists. */
+lg_core_error lg_backend_distill_grad(lg_ctx* ctx, void* stream, const lg_tensor* logits,
+                                      const lg_tensor* teacher_ids,
+                                      const lg_tensor* teacher_logprobs, const lg_tensor* weights,
+                                      float temperature, int32_t normalize,
+                                      const lg_tensor* losses, const lg_tensor* dlogits);
+
+/* ---------------------------------------------------------------------------------------
  * Wire format of stage boundaries (crates/core/src/lib.rs:298-412)
  *
  * "LNGL", u32 version 1, u32 dtype tag, u32 ndim (at most 8), ndim u32 extents, then the

@@ -41,6 +41,10 @@ SOURCES = [
     "permutation_kernels.hip",
     "training_kernels.hip",
     "backend_gemm16_kernels.hip",
+    "head.cpp",
+    "quantize_kernels.hip",
+    "gemm_blocks_kernels.hip",
+    "logits_kernels.hip",
 ]
 
 COMMON = ["-O3", "-std=c++17", "-fPIC", "-Wall", "-Wno-unused-function",

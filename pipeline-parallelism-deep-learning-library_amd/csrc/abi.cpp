@@ -165,6 +165,12 @@ void set_device(const lg_ctx* ctx) {
     if (ctx == nullptr) fail_invalid("null context");
     check_hip(hipSetDevice(ctx->device), "hipSetDevice");
 }
+
+bool capturing(hipStream_t s) {
+    hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+    check_hip(hipStreamIsCapturing(s, &st), "hipStreamIsCapturing");
+    return st != hipStreamCaptureStatusNone;
+}
 }  // namespace lg
 
 using namespace lg;

@@ -13,17 +13,10 @@
 //   Shape             C reaches past its storage (when M, N > 0); A or B reach past theirs
 //                     (when alpha != 0 and K > 0)
 // Then f32 runs on the device; F16 and BF16 report UnsupportedDevice (not built here).
-#include "lg_internal.h"
+#include "tensor_checks.h"
 
 namespace lg {
 namespace {
-
-struct TensorErr {
-    lg_core_error code;
-    std::string message;
-};
-
-[[noreturn]] void core_fail(lg_core_error code, const std::string& msg) { throw TensorErr{code, msg}; }
 
 uint64_t dtype_size(uint32_t dtype) {
     switch (dtype) {
@@ -174,40 +167,6 @@ uint64_t prepare_f32_row_major(std::initializer_list<const lg_tensor*> ts) {
         if (t->bytes < count * 4) core_fail(LG_CORE_SHAPE, "operand reaches past its storage");
     }
     return count;
-}
-
-// Runs `body` (checks, then launches) with the entry points' error mapping: check failures
-// return their code; device failures return UnsupportedDevice with the HIP message.
-template <typename F>
-lg_core_error run_op(F&& body) {
-    try {
-        body();
-        clear_last_error();
-        return LG_CORE_OK;
-    } catch (const TensorErr& e) {
-        set_last_error(e.message);
-        return e.code;
-    } catch (const Failure& f) {
-        set_last_error(f.message);
-        return LG_CORE_UNSUPPORTED_DEVICE;
-    } catch (const std::exception& e) {
-        set_last_error(e.what());
-        return LG_CORE_UNSUPPORTED_DEVICE;
-    } catch (...) {
-        set_last_error("internal error: unknown exception");
-        return LG_CORE_UNSUPPORTED_DEVICE;
-    }
-}
-
-hipStream_t device_stream(lg_ctx* ctx, void* stream) {
-    if (ctx == nullptr) core_fail(LG_CORE_UNSUPPORTED_DEVICE, "null context");
-    set_device(ctx);
-    return pick_stream(ctx, stream);
-}
-
-template <typename T>
-T* dev(const lg_tensor* t) {
-    return static_cast<T*>(t->base);
 }
 
 }  // namespace

@@ -1192,12 +1192,6 @@ struct Scratch {
     uint32_t* counters = nullptr;  // stream-K tickets, SK_COUNTER_BYTES after the partials
 };
 
-bool capturing(hipStream_t s) {
-    hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
-    check_hip(hipStreamIsCapturing(s, &st), "hipStreamIsCapturing");
-    return st != hipStreamCaptureStatusNone;
-}
-
 bool needs_scratch(const Plan& p) {
     return !p.half && (p.info.kind == LG_PLAN_SPLIT || (p.info.kind == LG_PLAN_DOT && p.dot.splits > 1) ||
                        (p.info.kind == LG_PLAN_TILED && p.gemm.kernel == KERN_SK));
@@ -1266,33 +1260,7 @@ void execute(lg_ctx* ctx, hipStream_t s, Plan& p) {
         launch_plan(ctx, s, p, Scratch{});
         return;
     }
-    // The context's scratch, made with the context and never grown, so this path allocates
-    // nothing and never blocks. Eager calls are ordered after the previous user: calls on the
-    // context's own stream by the stream, any other pair by split_event (also when both are
-    // one caller's stream handle: the handle may name a new stream created after the old one
-    // was destroyed with work still queued). A call under stream capture cannot wait on or
-    // record an eager event; it is ordered only by its own stream, so replays of the graph
-    // must not overlap the context's other split work (the caller orders them).
-    std::lock_guard<std::mutex> hold(ctx->split_lock);
-    const bool cap = capturing(s);
-    if (!cap) {
-        const bool own = s == ctx->stream && ctx->split_stream == ctx->stream;
-        if (ctx->split_stream != nullptr && !own) {
-            if (ctx->split_stream == ctx->stream) {
-                check_hip(hipEventRecord(ctx->split_event, ctx->stream), "hipEventRecord");
-            }
-            check_hip(hipStreamWaitEvent(s, ctx->split_event, 0), "hipStreamWaitEvent");
-        }
-    }
-    launch_plan(ctx, s, p, scratch_at(ctx->split_scratch));
-    if (!cap) {
-        ctx->split_stream = s;
-        if (s != ctx->stream) {
-            // Marks the end of this use for a later call on another stream; the context's own
-            // stream outlives the buffer, so its uses are marked only when needed.
-            check_hip(hipEventRecord(ctx->split_event, s), "hipEventRecord");
-        }
-    }
+    with_split_scratch(ctx, s, [&](void* scratch) { launch_plan(ctx, s, p, scratch_at(scratch)); });
 }
 
 void run(lg_ctx* ctx, void* stream, Plan plan, bool wait) {

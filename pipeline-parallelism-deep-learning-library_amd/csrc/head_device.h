@@ -1,0 +1,115 @@
+// Device helpers of the head's kernels: 16-bit and f32 elements in runs of eight, at any alignment.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include "head.h"
+
+namespace lg {
+namespace head_detail {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+// Vectors in memory at any byte address: gfx950 loads and stores them whole, aligned or not.
+typedef u32x2 u32x2_any __attribute__((aligned(1)));
+typedef u32x4 u32x4_any __attribute__((aligned(1)));
+
+template <uint32_t DT>
+constexpr uint32_t elem_size = DT == LG_DTYPE_F32 ? 4 : 2;
+
+// One element as f32, from its bits.
+template <uint32_t DT>
+__device__ inline float widen(uint32_t bits) {
+    if constexpr (DT == LG_DTYPE_F32) {
+        return __uint_as_float(bits);
+    } else if constexpr (DT == LG_DTYPE_BF16) {
+        return __uint_as_float(bits << 16);
+    } else {
+        return static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(bits)));
+    }
+}
+
+// One element at p; the address is a multiple of the element's size.
+template <uint32_t DT>
+__device__ inline float load_one(const char* p) {
+    if constexpr (DT == LG_DTYPE_F32) {
+        return *reinterpret_cast<const float*>(p);
+    } else {
+        return widen<DT>(*reinterpret_cast<const uint16_t*>(p));
+    }
+}
+
+template <uint32_t DT>
+__device__ inline void store_one(char* p, float v) {
+    if constexpr (DT == LG_DTYPE_F32) {
+        *reinterpret_cast<float*>(p) = v;
+    } else if constexpr (DT == LG_DTYPE_BF16) {
+        *reinterpret_cast<__bf16*>(p) = static_cast<__bf16>(v);  // to nearest, ties to even
+    } else {
+        *reinterpret_cast<_Float16*>(p) = static_cast<_Float16>(v);
+    }
+}
+
+// Eight consecutive elements as they lie in memory.
+template <uint32_t DT>
+struct Run {
+    u32x4 w[elem_size<DT> / 2];
+
+    __device__ inline void load(const char* p) {
+#pragma unroll
+        for (int i = 0; i < static_cast<int>(elem_size<DT> / 2); ++i) w[i] = *reinterpret_cast<const u32x4_any*>(p + 16 * i);
+    }
+    __device__ inline float operator[](int e) const {
+        if constexpr (DT == LG_DTYPE_F32) {
+            return __uint_as_float(w[e / 4][e % 4]);
+        } else if constexpr (DT == LG_DTYPE_BF16) {
+            const uint32_t v = w[0][e / 2];
+            return __uint_as_float(e % 2 ? v & 0xffff0000u : v << 16);
+        } else {
+            const uint32_t v = w[0][e / 2];
+            return widen<DT>(e % 2 ? v >> 16 : v & 0xffffu);
+        }
+    }
+};
+
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+
+// Two f32 values rounded to the 16-bit type, to nearest, ties to even, in one word.
+template <uint32_t DT>
+__device__ inline uint32_t pack2(float a, float b) {
+    if constexpr (DT == LG_DTYPE_BF16) {
+        const bf16x2 v = {static_cast<__bf16>(a), static_cast<__bf16>(b)};
+        return __builtin_bit_cast(uint32_t, v);
+    } else {
+        const f16x2 v = {static_cast<_Float16>(a), static_cast<_Float16>(b)};
+        return __builtin_bit_cast(uint32_t, v);
+    }
+}
+
+template <uint32_t DT>
+__device__ inline void store_run(char* p, const float (&v)[8]) {
+    if constexpr (DT == LG_DTYPE_F32) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            u32x4 o;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] = __float_as_uint(v[4 * i + e]);
+            *reinterpret_cast<u32x4_any*>(p + 16 * i) = o;
+        }
+    } else {
+        u32x4 o;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = pack2<DT>(v[2 * e], v[2 * e + 1]);
+        *reinterpret_cast<u32x4_any*>(p) = o;
+    }
+}
+
+inline void launched(Context* ctx, const char* name) {
+    check_hip(hipGetLastError(), name);
+    note_launch(ctx, name);
+}
+
+}  // namespace head_detail
+}  // namespace lg

@@ -424,4 +424,36 @@ void noalloc_prepare(lg_ctx* ctx);
 inline hipStream_t pick_stream(const lg_ctx* ctx, void* stream) {
     return stream ? static_cast<hipStream_t>(stream) : ctx->stream;
 }
+bool capturing(hipStream_t s);  // whether the stream is being captured
+
+// Hands the context's split scratch to `launches`, which enqueues its users on `s`. The scratch
+// is made with the context and never grown, so this allocates nothing and never blocks. Eager
+// calls are ordered after the previous user: calls on the context's own stream by the stream, any
+// other pair by split_event (also when both are one caller's stream handle: the handle may name a
+// new stream created after the old one was destroyed with work still queued). A call under stream
+// capture cannot wait on or record an eager event; it is ordered only by its own stream, so
+// replays of the graph must not overlap the context's other split work (the caller orders them).
+template <typename F>
+void with_split_scratch(lg_ctx* ctx, hipStream_t s, F&& launches) {
+    std::lock_guard<std::mutex> hold(ctx->split_lock);
+    const bool cap = capturing(s);
+    if (!cap) {
+        const bool own = s == ctx->stream && ctx->split_stream == ctx->stream;
+        if (ctx->split_stream != nullptr && !own) {
+            if (ctx->split_stream == ctx->stream) {
+                check_hip(hipEventRecord(ctx->split_event, ctx->stream), "hipEventRecord");
+            }
+            check_hip(hipStreamWaitEvent(s, ctx->split_event, 0), "hipStreamWaitEvent");
+        }
+    }
+    launches(ctx->split_scratch);
+    if (!cap) {
+        ctx->split_stream = s;
+        if (s != ctx->stream) {
+            // Marks the end of this use for a later call on another stream; the context's own
+            // stream outlives the buffer, so its uses are marked only when needed.
+            check_hip(hipEventRecord(ctx->split_event, s), "hipEventRecord");
+        }
+    }
+}
 }  // namespace lg

@@ -1,0 +1,811 @@
+// gfx950 kernels over rows of logits: log probabilities with entropy and top alternatives, their
+// gradient, and distillation's loss and gradient.
+//
+// One pass reads a row once: each thread keeps a running maximum m and, relative to it, s = sum of
+// 2^d and u = sum of 2^d d with d = (x - m) log2(e) / T, rescaled when m grows; sums of eight elements
+// are f32, everything above them f64, so a row whose probability lies on one element keeps the digits of
+// its small entropy. With the row's own m, s and u: log sum = ln s, entropy = ln 2 (log2 s - u / s). An
+// element of -inf gives s nothing, and u nothing because d is taken as -200 at the least; a NaN or +inf
+// makes s a NaN, which is how a row that has no distribution is told.
+//
+// A row is read in slots of eight elements that start at 16-byte boundaries of memory, whatever the
+// row's own alignment; the slots at its ends are read element by element. Rows are split over workgroups
+// where there are few of them; the workgroup that finishes a row last (a ticket) joins its parts in their
+// order. Nothing waits on another workgroup.
+#include <algorithm>
+
+#include "head_device.h"
+
+namespace lg {
+namespace {
+
+using namespace head_detail;
+
+constexpr int THREADS = 512;
+constexpr int WAVES = THREADS / 64;
+constexpr int UNROLL = 4;               // slots a thread loads before it uses the first
+constexpr uint32_t MAX_LIST = 512;      // slots whose elements are looked at for the alternatives
+constexpr uint32_t MAX_KEYS = 8 * MAX_LIST;
+constexpr uint32_t SLOT_BYTES = 32768;  // LDS of the slots' maxima: 2 or 4 bytes each
+constexpr uint32_t TICKETS = SK_COUNTER_BYTES / sizeof(uint32_t);
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr double LN2 = 0.69314718055994530942;
+constexpr float INF = __builtin_inff();
+constexpr float FAR = -200.0f;  // below it 2^d is zero in f32
+
+__device__ inline float exp2_fast(float d) { return __builtin_amdgcn_exp2f(d); }
+
+// A row's m and, relative to it, s and u; or those of a part of it.
+struct Part {
+    float m;
+    float pad;
+    double s, u;
+};
+
+// What a pass leaves of a row for its gradient.
+struct RowInfo {
+    float m, log2s;
+    float scale;  // the gradient is scale * p_j less the teacher's; 0: all zeros; NaN: all NaN
+    float norm;   // log of the teacher's normalizer
+};
+
+struct PassArgs {
+    const char* x;
+    int64_t x_pitch;
+    uint32_t row0, cols;
+    uint32_t segs, seg_slots;  // workgroups to a row, slots to a workgroup
+    float c, temperature;      // log2(e) / temperature
+    Part* parts;               // [row - row0][segs]
+    uint64_t* part_keys;       // [row - row0][segs][k]
+    uint32_t* tickets;         // zero between launches
+    LogprobArgs lp;
+    DistillArgs ds;
+    RowInfo* info;  // [row - row0], or null
+};
+
+// A row's slots.
+template <uint32_t DT>
+struct Slots {
+    const char* base;  // of slot 0: the row's start rounded down to 16 bytes
+    uint32_t head;     // elements of slot 0 before the row
+    uint32_t cols, count;
+
+    __device__ inline Slots(const char* row, uint32_t n) {
+        head = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(row) & 15) / elem_size<DT>;
+        base = row - head * elem_size<DT>;
+        cols = n;
+        count = n == 0 ? 0 : (head + n + 7) / 8;
+    }
+    // Index in the row of slot j's first element, negative for one before it.
+    __device__ inline int64_t first(uint32_t j) const { return static_cast<int64_t>(j) * 8 - head; }
+    __device__ inline bool whole(uint32_t j) const { return first(j) >= 0 && first(j) + 8 <= cols; }
+    // Slot j; what lies outside the row is -inf.
+    __device__ inline void load(uint32_t j, Run<DT>& r) const {
+        if (whole(j)) {
+            r.load(base + static_cast<uint64_t>(j) * 8 * elem_size<DT>);
+            return;
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const int64_t i = first(j) + e;
+            const char* p = base + (static_cast<uint64_t>(j) * 8 + e) * elem_size<DT>;
+            const bool inside = i >= 0 && i < cols;
+            if constexpr (DT == LG_DTYPE_F32) {
+                r.w[e / 4][e % 4] = inside ? *reinterpret_cast<const uint32_t*>(p) : 0xff800000u;
+            } else {
+                const uint32_t none = DT == LG_DTYPE_BF16 ? 0xff80u : 0xfc00u;
+                const uint32_t bits = inside ? *reinterpret_cast<const uint16_t*>(p) : none;
+                r.w[0][e / 2] = e % 2 ? (r.w[0][e / 2] & 0xffffu) | bits << 16 : bits;
+            }
+        }
+    }
+};
+
+// A slot's maximum in LDS: its own 16 bits, or f32.
+template <uint32_t DT>
+struct SlotMax {
+    typedef uint16_t T;
+    static __device__ inline T pack(float v) {
+        if constexpr (DT == LG_DTYPE_BF16) {
+            return static_cast<uint16_t>(__float_as_uint(v) >> 16);
+        } else {
+            return __builtin_bit_cast(uint16_t, static_cast<_Float16>(v));
+        }
+    }
+    static __device__ inline float unpack(T b) { return widen<DT>(b); }
+};
+template <>
+struct SlotMax<LG_DTYPE_F32> {
+    typedef float T;
+    static __device__ inline T pack(float v) { return v; }
+    static __device__ inline float unpack(T b) { return b; }
+};
+
+// f32 as whole numbers of the same order; -0 counts as +0. No number gives 0.
+__device__ inline uint32_t order(float v) {
+    const uint32_t b = __float_as_uint(v + 0.0f);
+    return b ^ (b >> 31 ? 0xffffffffu : 0x80000000u);
+}
+__device__ inline float unorder(uint32_t o) { return __uint_as_float(o >> 31 ? o ^ 0x80000000u : ~o); }
+// Larger for a larger logit, and for a lower index among equal ones.
+__device__ inline uint64_t key_of(float v, uint32_t index) { return static_cast<uint64_t>(order(v)) << 32 | (0xffffffffu - index); }
+__device__ inline float key_value(uint64_t k) { return unorder(static_cast<uint32_t>(k >> 32)); }
+__device__ inline uint32_t key_index(uint64_t k) { return 0xffffffffu - static_cast<uint32_t>(k); }
+
+struct Shared {
+    alignas(16) uint64_t wide[SLOT_BYTES / 8];  // the slots' maxima, then the candidates' keys
+    uint64_t best[TOP_MAX];
+    float tops[THREADS];
+    uint32_t list[MAX_LIST];
+    double s[WAVES], u[WAVES];
+    float m[WAVES];
+    uint32_t count, limit;
+    Part row;
+    bool last;
+};
+static_assert(MAX_KEYS * sizeof(uint64_t) <= SLOT_BYTES, "the keys take the maxima's place");
+
+// The largest of `tops` that at least k of them reach, to sixteen bits of its order and from below;
+// -inf where fewer than k are above -inf. By one wave.
+__device__ inline float threshold(const float* tops, uint32_t k) {
+    const uint32_t lane = threadIdx.x % 64;
+    uint32_t o[THREADS / 64];
+#pragma unroll
+    for (int i = 0; i < THREADS / 64; ++i) o[i] = order(tops[i * 64 + lane]) >> 16;
+    uint32_t t = 0;
+    for (uint32_t bit = 0x8000u; bit != 0; bit >>= 1) {
+        const uint32_t at = t | bit;
+        uint32_t n = 0;
+#pragma unroll
+        for (int i = 0; i < THREADS / 64; ++i) n += __popcll(__ballot(o[i] >= at));
+        if (n >= k) t = at;
+    }
+    const float v = unorder(t << 16);
+    return t <= 0x007fu ? -INF : v;
+}
+
+// How many of the workgroup's threads' `mine` there are in all.
+__device__ inline uint32_t total(Shared& sh, uint32_t mine) {
+    __syncthreads();
+    if (threadIdx.x == 0) sh.count = 0;
+    __syncthreads();
+    if (mine) atomicAdd(&sh.count, mine);
+    __syncthreads();
+    return sh.count;
+}
+
+// sh.best = the k largest of the n keys in sh.wide, in order, then zeros. Keys differ from one another.
+__device__ inline void rank_keys(Shared& sh, uint32_t n, uint32_t k) {
+    for (uint32_t i = threadIdx.x; i < k; i += THREADS) sh.best[i] = 0;
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < n; i += THREADS) {
+        const uint64_t mine = sh.wide[i];
+        uint32_t above = 0;
+        for (uint32_t j = 0; j < n; ++j) above += sh.wide[j] > mine ? 1 : 0;
+        if (above < k) sh.best[above] = mine;
+    }
+    __syncthreads();
+}
+
+// sh.best = the k largest keys of slots [lo, hi), whose maxima are in sh.wide and whose threads' maxima
+// are `mine`. An alternative lies in a slot whose maximum is one of the k largest, so slots below the
+// k-th largest of the threads' maxima drop out. Should more than MAX_LIST slots remain (many equal
+// logits), the k-th largest slot itself is found, bit by bit, with the slots that equal it taken from the
+// lowest.
+template <uint32_t DT>
+__device__ void top_of_slots(Shared& sh, const Slots<DT>& row, uint32_t lo, uint32_t hi, float mine, uint32_t k) {
+    typedef SlotMax<DT> Max;
+    const typename Max::T* maxima = reinterpret_cast<const typename Max::T*>(sh.wide);
+    const uint32_t tid = threadIdx.x, n = hi - lo;
+    sh.tops[tid] = mine;
+    if (tid == 0) sh.count = 0;
+    __syncthreads();
+    if (tid < 64) {
+        const float t = threshold(sh.tops, k);
+        if (tid == 0) sh.tops[0] = t;
+    }
+    __syncthreads();
+    float t = sh.tops[0];
+    if (mine >= t) {
+        for (uint32_t i = tid; i < n; i += THREADS) {
+            const float v = Max::unpack(maxima[i]);
+            if (v >= t && v > -INF) {
+                const uint32_t at = atomicAdd(&sh.count, 1u);
+                if (at < MAX_LIST) sh.list[at] = i;
+            }
+        }
+    }
+    __syncthreads();
+    uint32_t listed = sh.count;
+    if (listed > MAX_LIST) {
+        uint32_t o = 0;
+        for (uint32_t bit = 0x80000000u; bit != 0; bit >>= 1) {
+            uint32_t c = 0;
+            for (uint32_t i = tid; i < n; i += THREADS) c += order(Max::unpack(maxima[i])) >= (o | bit) ? 1 : 0;
+            if (total(sh, c) >= k) o |= bit;
+        }
+        uint32_t c = 0;
+        for (uint32_t i = tid; i < n; i += THREADS) c += order(Max::unpack(maxima[i])) > o ? 1 : 0;
+        const uint32_t equal = k - total(sh, c);  // wanted from the slots whose maximum is the k-th: at least one
+        uint32_t end = 0;                         // slots below `end` hold fewer of them than that
+        for (uint32_t bit = 0x80000000u; bit != 0; bit >>= 1) {
+            const uint32_t at = end | bit;
+            if (at > n) continue;
+            c = 0;
+            for (uint32_t i = tid; i < at; i += THREADS) c += order(Max::unpack(maxima[i])) == o ? 1 : 0;
+            if (total(sh, c) < equal) end = at;
+        }
+        t = unorder(o);
+        __syncthreads();
+        if (tid == 0) sh.count = 0;
+        __syncthreads();
+        for (uint32_t i = tid; i < n; i += THREADS) {
+            const float v = Max::unpack(maxima[i]);
+            if (order(v) > o || (order(v) == o && i <= end)) sh.list[atomicAdd(&sh.count, 1u)] = i;
+        }
+        __syncthreads();
+        listed = sh.count;  // k
+    }
+    __syncthreads();
+    if (tid == 0) sh.count = 0;
+    __syncthreads();
+    for (uint32_t i = tid; i < listed * 8; i += THREADS) {
+        const uint32_t j = lo + sh.list[i / 8];
+        const int64_t index = row.first(j) + i % 8;
+        if (index < 0 || index >= row.cols) continue;
+        const float v = load_one<DT>(row.base + (static_cast<uint64_t>(j) * 8 + i % 8) * elem_size<DT>);
+        if (v >= t && v > -INF) sh.wide[atomicAdd(&sh.count, 1u)] = key_of(v, static_cast<uint32_t>(index));
+    }
+    __syncthreads();
+    rank_keys(sh, sh.count, k);
+}
+
+// The joined sums of the workgroup's threads, each relative to its own m.
+__device__ inline Part join(Shared& sh, float m, double s, double u, float c) {
+    const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+    float top = m;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
+    __syncthreads();
+    if (lane == 0) sh.m[wave] = top;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) top = fmaxf(top, sh.m[w]);
+    if (m != -INF) {  // else s and u are zero, or NaN
+        const float shift = (m - top) * c;
+        const double f = exp2_fast(shift);
+        u = f * (u + fmaxf(shift, 4 * FAR) * s);
+        s = f * s;
+    }
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+        s += __shfl_xor(s, d);
+        u += __shfl_xor(u, d);
+    }
+    if (lane == 0) {
+        sh.s[wave] = s;
+        sh.u[wave] = u;
+    }
+    __syncthreads();
+    Part p{top, 0.0f, 0.0, 0.0};
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) {
+        p.s += sh.s[w];
+        p.u += sh.u[w];
+    }
+    return p;
+}
+
+// Writes what is asked of a row with sums p and, for k > 0, its best keys in sh.best.
+template <uint32_t DT>
+__device__ inline void finish_logprobs(const PassArgs& a, const Shared& sh, const char* x, uint32_t row, Part p) {
+    const LogprobArgs& o = a.lp;
+    const uint32_t tid = threadIdx.x;
+    const bool bad = p.s != p.s, empty = !bad && p.m == -INF;
+    const double log_s = empty ? 0.0 : log(p.s);
+    const float nan = __builtin_nanf("");
+    if (tid == 0) {
+        if (o.tokens != nullptr) {
+            const int32_t t = o.tokens[row];
+            float v = 0.0f;
+            if (t >= 0 && static_cast<uint32_t>(t) < a.cols) {
+                const float d = load_one<DT>(x + static_cast<uint64_t>(t) * elem_size<DT>) - (empty ? 0.0f : p.m);
+                v = bad ? nan : static_cast<float>(static_cast<double>(d) / o.temperature - log_s);
+            }
+            o.logprobs[row] = v;
+        }
+        if (o.entropy != nullptr) o.entropy[row] = bad ? nan : empty ? 0.0f : static_cast<float>(log_s - LN2 * (p.u / p.s));
+        if (o.stats != nullptr) {
+            o.stats[row * o.stats_pitch] = bad ? nan : p.m;
+            o.stats[row * o.stats_pitch + 1] = bad ? nan : empty ? -INF : static_cast<float>(log_s);
+        }
+    }
+    for (uint32_t i = tid; i < o.k; i += THREADS) {
+        const uint64_t key = bad ? 0 : sh.best[i];
+        o.top_ids[row * o.ids_pitch + i] = key == 0 ? -1 : static_cast<int32_t>(key_index(key));
+        const float v = key == 0 ? -INF : static_cast<float>(static_cast<double>(key_value(key) - p.m) / o.temperature - log_s);
+        o.top[row * o.top_pitch + i] = bad ? nan : v;
+    }
+}
+
+// Whether entry i of a row's list names one of `cols` logits with a probability, and its log.
+struct Teacher {
+    const int32_t* ids;
+    const float* values;
+    uint32_t k, cols;
+    __device__ inline Teacher(const DistillArgs& a, uint32_t row) {
+        ids = a.ids + row * a.ids_pitch;
+        values = a.values + row * a.values_pitch;
+        k = a.k;
+        cols = a.cols;
+    }
+    __device__ inline bool named(uint32_t i, uint32_t* id, float* value) const {
+        if (i >= k || ids[i] < 0 || static_cast<uint32_t>(ids[i]) >= cols || values[i] == -INF) return false;
+        *id = static_cast<uint32_t>(ids[i]);
+        *value = values[i];
+        return true;
+    }
+};
+
+// A row's loss and what its gradient needs, by one wave: each lane takes two of the list's entries.
+template <uint32_t DT>
+__device__ inline RowInfo finish_distill(const PassArgs& a, const char* x, uint32_t row, Part p) {
+    const DistillArgs& o = a.ds;
+    const uint32_t lane = threadIdx.x % 64;
+    const bool bad = p.s != p.s, empty = !bad && p.m == -INF;
+    const float weight = (o.weights != nullptr ? o.weights[row] : 1.0f) * o.temperature;
+    const Teacher teacher(o, row);
+    uint32_t id[2] = {0, 0};
+    float value[2] = {-INF, -INF};
+    bool named[2];
+    float top = -INF;
+    for (int i = 0; i < 2; ++i) {
+        named[i] = teacher.named(lane + 64 * i, &id[i], &value[i]);
+        if (named[i]) top = fmaxf(top, value[i]);
+    }
+    const bool any = __ballot(named[0] || named[1]) != 0;
+    double norm = 0.0;
+    if (o.normalize) {
+        for (int d = 1; d < 64; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
+        double sum = 0.0;
+        for (int i = 0; i < 2; ++i) {
+            if (named[i]) sum += exp(static_cast<double>(value[i]) - top);
+        }
+        for (int d = 1; d < 64; d *= 2) sum += __shfl_xor(sum, d);
+        norm = top + log(sum);
+    }
+    const double log_s = empty ? 0.0 : log(p.s);
+    double mass = 0.0, loss = 0.0;
+    for (int i = 0; i < 2; ++i) {
+        if (!named[i] || empty) continue;
+        const double lp = value[i] - norm, q = exp(lp);
+        mass += q;
+        const float d = load_one<DT>(x + static_cast<uint64_t>(id[i]) * elem_size<DT>) - p.m;
+        if (q != 0.0) loss += q * (lp - (static_cast<double>(d) / o.temperature - log_s));
+    }
+    for (int d = 1; d < 64; d *= 2) {
+        mass += __shfl_xor(mass, d);
+        loss += __shfl_xor(loss, d);
+    }
+    const bool idle = empty || weight == 0.0f || !any;
+    const float nan = __builtin_nanf("");
+    if (lane == 0) o.losses[row] = idle ? 0.0f : bad ? nan : static_cast<float>(loss * weight * o.temperature);
+    return RowInfo{p.m, static_cast<float>(log_s / LN2), idle ? 0.0f : bad ? nan : static_cast<float>(mass * weight), static_cast<float>(norm)};
+}
+
+// One workgroup's part of one row; the row's last workgroup finishes it.
+template <uint32_t DT, bool ENTROPY, bool TOP, bool DISTILL>
+__global__ __launch_bounds__(THREADS) void row_pass(PassArgs a) {
+    __shared__ Shared sh;
+    const uint32_t tid = threadIdx.x, at = blockIdx.x / a.segs, seg = blockIdx.x % a.segs, row = a.row0 + at;
+    const char* x = a.x + row * a.x_pitch * elem_size<DT>;
+    if constexpr (DISTILL) {
+        if (a.ds.weights != nullptr && a.ds.weights[row] == 0.0f) {  // a row without weight is not read
+            if (tid == 0 && seg == 0) {
+                a.ds.losses[row] = 0.0f;
+                if (a.info != nullptr) a.info[at] = RowInfo{0.0f, 0.0f, 0.0f, 0.0f};
+            }
+            return;
+        }
+    }
+    const Slots<DT> slots(x, a.cols);
+    const uint32_t lo = min(seg * a.seg_slots, slots.count), hi = min(lo + a.seg_slots, slots.count);
+    typename SlotMax<DT>::T* maxima = reinterpret_cast<typename SlotMax<DT>::T*>(sh.wide);
+    float m = -INF;
+    double s = 0.0, u = 0.0;
+    for (uint32_t j0 = lo + tid; j0 < hi; j0 += THREADS * UNROLL) {
+        Run<DT> r[UNROLL];
+#pragma unroll
+        for (int i = 0; i < UNROLL; ++i) {
+            const uint32_t j = j0 + i * THREADS;
+            if (j < hi) {
+                slots.load(j, r[i]);
+            } else {
+                const uint32_t none = DT == LG_DTYPE_F32 ? 0xff800000u : DT == LG_DTYPE_BF16 ? 0xff80ff80u : 0xfc00fc00u;
+#pragma unroll
+                for (int w = 0; w < static_cast<int>(elem_size<DT> / 2); ++w) r[i].w[w] = u32x4{none, none, none, none};
+            }
+        }
+        float top = m;
+#pragma unroll
+        for (int i = 0; i < UNROLL; ++i) {
+            float v = r[i][0];
+#pragma unroll
+            for (int e = 1; e < 8; ++e) v = fmaxf(v, r[i][e]);
+            if (TOP && j0 + i * THREADS < hi) maxima[j0 + i * THREADS - lo] = SlotMax<DT>::pack(v);
+            top = fmaxf(top, v);
+        }
+        const float ref = top == -INF ? 0.0f : top, shift = fmaxf((m - ref) * a.c, 4 * FAR);
+        const double f = exp2_fast(shift);
+        u = f * (u + shift * s);
+        s = f * s;
+#pragma unroll
+        for (int i = 0; i < UNROLL; ++i) {
+            float ps = 0.0f, pu = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float d = (r[i][e] - ref) * a.c, p = exp2_fast(d);
+                ps += p;
+                if (ENTROPY) pu = __builtin_fmaf(p, fmaxf(d, FAR), pu);
+            }
+            s += ps;
+            if (ENTROPY) u += pu;
+        }
+        m = top;
+    }
+    Part p = join(sh, m, s, u, a.c);
+    if constexpr (TOP) top_of_slots<DT>(sh, slots, lo, hi, m, a.lp.k);
+    if (a.segs > 1) {
+        // Thread 0 writes the part and draws the ticket; the keys are wave 0's.
+        if (tid < 64) {
+            if constexpr (TOP) {
+                uint64_t* keys = a.part_keys + (static_cast<uint64_t>(at) * a.segs + seg) * a.lp.k;
+                for (uint32_t i = tid; i < a.lp.k; i += 64) __hip_atomic_store(keys + i, sh.best[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            }
+            if (tid == 0) {
+                Part* to = a.parts + static_cast<uint64_t>(at) * a.segs + seg;
+                __hip_atomic_store(&to->m, p.m, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                __hip_atomic_store(&to->s, p.s, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                __hip_atomic_store(&to->u, p.u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            }
+            __threadfence();
+            if (tid == 0) sh.last = __hip_atomic_fetch_add(a.tickets + at, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == a.segs - 1;
+        }
+        __syncthreads();
+        if (!sh.last) return;
+        __threadfence();
+        if (tid == 0) __hip_atomic_store(a.tickets + at, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        // Each thread joins the parts of its turn, in order.
+        float jm = -INF;
+        double js = 0.0, ju = 0.0;
+        for (uint32_t i = tid; i < a.segs; i += THREADS) {
+            const Part* q = a.parts + static_cast<uint64_t>(at) * a.segs + i;
+            const float qm = __hip_atomic_load(&q->m, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            const double qs = __hip_atomic_load(&q->s, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            const double qu = __hip_atomic_load(&q->u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            const float ref = fmaxf(jm, qm);
+            const float f = ref == -INF ? 0.0f : fmaxf((jm - ref) * a.c, 4 * FAR), g = ref == -INF ? 0.0f : fmaxf((qm - ref) * a.c, 4 * FAR);
+            ju = exp2_fast(f) * (ju + f * js) + exp2_fast(g) * (qu + g * qs);
+            js = exp2_fast(f) * js + exp2_fast(g) * qs;
+            jm = ref;
+        }
+        p = join(sh, jm, js, ju, a.c);
+        if constexpr (TOP) {
+            const uint32_t k = a.lp.k, all = a.segs * k;
+            const uint64_t* keys = a.part_keys + static_cast<uint64_t>(at) * all;
+            // Each part's first few keys bound the k-th of all from below.
+            const uint32_t each = min(k, THREADS / a.segs), sg = tid / each;
+            float v = -INF;
+            if (each > 0 && sg < a.segs) {
+                const uint64_t key = __hip_atomic_load(keys + sg * k + tid % each, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                if (key != 0) v = key_value(key);
+            }
+            sh.tops[tid] = v;
+            if (tid == 0) sh.count = 0;
+            __syncthreads();
+            if (tid < 64) {
+                const float t = threshold(sh.tops, k);
+                if (tid == 0) sh.tops[0] = t;
+            }
+            __syncthreads();
+            const float t = sh.tops[0];
+            for (uint32_t i = tid; i < all; i += THREADS) {
+                const uint64_t key = __hip_atomic_load(keys + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                if (key != 0 && key_value(key) >= t) sh.wide[atomicAdd(&sh.count, 1u)] = key;
+            }
+            __syncthreads();
+            rank_keys(sh, sh.count, k);
+        }
+    }
+    if constexpr (DISTILL) {
+        if (tid < 64) {
+            const RowInfo info = finish_distill<DT>(a, x, row, p);
+            if (a.info != nullptr && tid == 0) a.info[at] = info;
+        }
+    } else {
+        finish_logprobs<DT>(a, sh, x, row, p);
+    }
+}
+
+// ------------------------------------------------------------------------------- gradients
+
+constexpr int GRAD_THREADS = 256;
+constexpr int GRAD_UNROLL = 4;
+constexpr uint32_t GRAD_SLOTS = GRAD_THREADS * GRAD_UNROLL;  // of a workgroup
+
+struct GradArgs {
+    const char* x;
+    char* dx;
+    int64_t x_pitch, dx_pitch;
+    uint32_t row0, cols, segs;
+    float c, inverse;  // log2(e) / temperature, 1 / temperature
+    LogprobBackArgs lp;
+    DistillArgs ds;
+    const RowInfo* info;
+};
+
+enum GradMode { LOGPROB, LOGPROB_ENTROPY, TEACHER };
+
+// dx of GRAD_SLOTS slots of a row: an element at a time from the row's statistics. The token's own term
+// joins in its slot; a teacher's are written over the dense gradient when it is complete, from logits read before.
+template <uint32_t DT, GradMode MODE>
+__global__ __launch_bounds__(GRAD_THREADS) void grad_rows(GradArgs a) {
+    const uint32_t tid = threadIdx.x, at = blockIdx.x / a.segs, seg = blockIdx.x % a.segs, row = a.row0 + at;
+    const char* x = a.x + row * a.x_pitch * elem_size<DT>;
+    char* dx = a.dx + row * a.dx_pitch * elem_size<DT>;
+    const Slots<DT> slots(x, a.cols);
+    float m, log2s, g = 0.0f, h = 0.0f, entropy = 0.0f, scale = 1.0f;
+    int64_t token = -1;
+    if constexpr (MODE == TEACHER) {
+        const RowInfo info = a.info[at];
+        m = info.m;
+        log2s = info.log2s;
+        scale = info.scale;
+    } else {
+        m = a.lp.stats[row * a.lp.stats_pitch];
+        log2s = a.lp.stats[row * a.lp.stats_pitch + 1] * LOG2E;
+        if (m == -INF) scale = 0.0f;
+        token = a.lp.tokens[row];
+        if (token >= a.cols) token = -1;
+        if (token >= 0) g = a.lp.dlogprobs[row] * a.inverse;
+        if constexpr (MODE == LOGPROB_ENTROPY) {
+            h = a.lp.dentropy[row] * a.inverse;
+            entropy = a.lp.entropy[row];
+        }
+    }
+    // One slot's gradient, from its logits.
+    auto gradient = [&](const Run<DT>& r, int64_t first, float (&o)[8]) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float d = (r[e] - m) * a.c - log2s, p = exp2_fast(d);
+            if constexpr (MODE == TEACHER) {
+                o[e] = scale * p;
+            } else if constexpr (MODE == LOGPROB) {
+                o[e] = -g * p;
+            } else {
+                o[e] = -p * __builtin_fmaf(h, __builtin_fmaf(fmaxf(d, FAR), static_cast<float>(LN2), entropy), g);
+            }
+            if constexpr (MODE != TEACHER) {
+                if (first + e == token) o[e] += g;
+            }
+            if (scale == 0.0f) o[e] = 0.0f;
+        }
+    };
+    __shared__ uint32_t ids[TOP_MAX];
+    __shared__ float minus[TOP_MAX], own[TOP_MAX];
+    const uint32_t lo = seg * GRAD_SLOTS;
+    if constexpr (MODE == TEACHER) {
+        // The list's entries that lie in these slots: their probabilities, and their logits' own before any is overwritten.
+        if (tid < TOP_MAX) {
+            uint32_t id = 0xffffffffu;
+            float value = 0.0f;
+            const Teacher teacher(a.ds, row);
+            ids[tid] = 0xffffffffu;
+            if (scale != 0.0f && teacher.named(tid, &id, &value)) {
+                const float weight = (a.ds.weights != nullptr ? a.ds.weights[row] : 1.0f) * a.ds.temperature;
+                minus[tid] = weight * exp2_fast((value - a.info[at].norm) * LOG2E);
+                ids[tid] = id;
+                const uint32_t j = (id + slots.head) / 8;
+                if (j >= lo && j < lo + GRAD_SLOTS) {
+                    own[tid] = scale * exp2_fast((load_one<DT>(x + static_cast<uint64_t>(id) * elem_size<DT>) - m) * a.c - log2s);
+                }
+            }
+        }
+        __syncthreads();
+    }
+    Run<DT> r[GRAD_UNROLL];
+#pragma unroll
+    for (int i = 0; i < GRAD_UNROLL; ++i) {
+        const uint32_t j = lo + i * GRAD_THREADS + tid;
+        if (j < slots.count && scale != 0.0f) slots.load(j, r[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < GRAD_UNROLL; ++i) {
+        const uint32_t j = lo + i * GRAD_THREADS + tid;
+        if (j >= slots.count) break;
+        float o[8];
+        gradient(r[i], slots.first(j), o);
+        if (slots.whole(j)) {
+            store_run<DT>(dx + slots.first(j) * elem_size<DT>, o);
+        } else {
+            for (int e = 0; e < 8; ++e) {
+                const int64_t index = slots.first(j) + e;
+                if (index >= 0 && index < a.cols) store_one<DT>(dx + index * elem_size<DT>, o[e]);
+            }
+        }
+    }
+    if constexpr (MODE == TEACHER) {
+        if (scale == 0.0f) return;
+        __syncthreads();
+        if (tid < TOP_MAX && ids[tid] != 0xffffffffu) {
+            const uint32_t id = ids[tid], j = (id + slots.head) / 8;
+            if (j >= lo && j < lo + GRAD_SLOTS) {
+                // An id that the list holds twice loses the sum of both, in the list's order.
+                float v = 0.0f;
+                for (uint32_t i = 0; i < a.ds.k; ++i) v += ids[i] == id ? minus[i] : 0.0f;
+                store_one<DT>(dx + static_cast<uint64_t>(id) * elem_size<DT>, own[tid] - v);
+            }
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------- launches
+
+uint32_t ceil_div(uint64_t a, uint64_t b) { return static_cast<uint32_t>((a + b - 1) / b); }
+
+// Workgroups to a row: enough that rows of any number give every compute unit two, while each has at
+// least a slot for every thread; and where alternatives are wanted, no more slots than their maxima have
+// room for in LDS, and no more parts than the keys of.
+struct Split {
+    uint32_t segs, seg_slots;
+};
+Split split_rows(uint32_t rows, uint32_t cols, uint32_t size, uint32_t k) {
+    const uint32_t slots = ceil_div(static_cast<uint64_t>(cols) + 7, 8) + 1, most = SLOT_BYTES / size;
+    uint32_t segs = rows >= 512 ? 1 : ceil_div(512, rows);
+    segs = std::min(segs, ceil_div(slots, THREADS));
+    if (k > 0) {
+        segs = std::min(segs, MAX_KEYS / k);
+        segs = std::max(segs, ceil_div(slots, most));
+        if (static_cast<uint64_t>(segs) * k > MAX_KEYS) fail_invalid("token_logprobs: alternatives of so many logits do not fit");
+    }
+    const uint32_t each = ceil_div(slots, segs);
+    return {ceil_div(slots, each), each};
+}
+
+template <uint32_t DT, bool ENTROPY, bool TOP, bool DISTILL>
+void launch_pass(lg_ctx* ctx, hipStream_t s, const PassArgs& a, uint32_t rows) {
+    hipLaunchKernelGGL((row_pass<DT, ENTROPY, TOP, DISTILL>), dim3(rows * a.segs), dim3(THREADS), 0, s, a);
+    launched(ctx, DISTILL ? "row_pass_distill" : TOP ? "row_pass_top" : "row_pass");
+}
+
+// Rows in batches of `most`, and of no more than a launch's threads have 32-bit numbers for.
+template <typename F>
+void batches(uint32_t rows, uint64_t wgs_per_row, uint64_t most, F&& launch) {
+    const uint64_t batch = std::min<uint64_t>(most, (1ull << 22) / wgs_per_row);
+    if (batch == 0) fail_invalid("rows of so many logits do not fit a launch");
+    for (uint64_t r = 0; r < rows; r += batch) launch(static_cast<uint32_t>(r), static_cast<uint32_t>(std::min<uint64_t>(batch, rows - r)));
+}
+
+// Rows whose parts fit the scratch and whose tickets there are.
+uint64_t split_most(uint32_t segs, uint64_t bytes_per_row) {
+    return std::min<uint64_t>(SPLIT_PARTIAL_MAX / bytes_per_row, segs > 1 ? TICKETS : UINT32_MAX);
+}
+
+template <uint32_t DT>
+void logprobs_of(lg_ctx* ctx, hipStream_t s, const LogprobArgs& o) {
+    const Split split = split_rows(o.rows, o.cols, elem_size<DT>, o.k);
+    PassArgs a{};
+    a.x = static_cast<const char*>(o.x);
+    a.x_pitch = o.x_pitch;
+    a.cols = o.cols;
+    a.segs = split.segs;
+    a.seg_slots = split.seg_slots;
+    a.c = LOG2E / o.temperature;
+    a.temperature = o.temperature;
+    a.lp = o;
+    const auto run = [&](void* scratch) {
+        const uint64_t per_row = split.segs * (sizeof(Part) + o.k * sizeof(uint64_t));
+        batches(o.rows, split.segs, split.segs == 1 ? o.rows : split_most(split.segs, per_row), [&](uint32_t r, uint32_t n) {
+            a.row0 = r;
+            if (scratch != nullptr) {
+                a.tickets = reinterpret_cast<uint32_t*>(static_cast<char*>(scratch) + SPLIT_PARTIAL_MAX);
+                a.parts = static_cast<Part*>(scratch);
+                a.part_keys = reinterpret_cast<uint64_t*>(a.parts + static_cast<uint64_t>(n) * split.segs);
+            }
+            if (o.k > 0) {
+                o.entropy != nullptr ? launch_pass<DT, true, true, false>(ctx, s, a, n) : launch_pass<DT, false, true, false>(ctx, s, a, n);
+            } else {
+                o.entropy != nullptr ? launch_pass<DT, true, false, false>(ctx, s, a, n) : launch_pass<DT, false, false, false>(ctx, s, a, n);
+            }
+        });
+    };
+    if (split.segs == 1) {
+        run(nullptr);
+    } else {
+        with_split_scratch(ctx, s, run);
+    }
+}
+
+template <uint32_t DT, GradMode MODE>
+void launch_grad(lg_ctx* ctx, hipStream_t s, const GradArgs& a, uint32_t rows) {
+    hipLaunchKernelGGL((grad_rows<DT, MODE>), dim3(rows * a.segs), dim3(GRAD_THREADS), 0, s, a);
+    launched(ctx, MODE == TEACHER ? "grad_rows_distill" : "grad_rows");
+}
+
+uint32_t grad_segs(uint32_t cols) { return ceil_div((static_cast<uint64_t>(cols) + 7 + 7) / 8, GRAD_SLOTS); }
+
+template <uint32_t DT>
+void back_of(lg_ctx* ctx, hipStream_t s, const LogprobBackArgs& o) {
+    GradArgs a{};
+    a.x = static_cast<const char*>(o.x);
+    a.dx = static_cast<char*>(o.dx);
+    a.x_pitch = o.x_pitch;
+    a.dx_pitch = o.dx_pitch;
+    a.cols = o.cols;
+    a.segs = grad_segs(o.cols);
+    a.c = LOG2E / o.temperature;
+    a.inverse = 1.0f / o.temperature;
+    a.lp = o;
+    batches(o.rows, a.segs, o.rows, [&](uint32_t r, uint32_t n) {
+        a.row0 = r;
+        o.dentropy != nullptr ? launch_grad<DT, LOGPROB_ENTROPY>(ctx, s, a, n) : launch_grad<DT, LOGPROB>(ctx, s, a, n);
+    });
+}
+
+template <uint32_t DT>
+void distill_of(lg_ctx* ctx, hipStream_t s, const DistillArgs& o) {
+    const Split split = split_rows(o.rows, o.cols, elem_size<DT>, 0);
+    PassArgs a{};
+    a.x = static_cast<const char*>(o.x);
+    a.x_pitch = o.x_pitch;
+    a.cols = o.cols;
+    a.segs = split.segs;
+    a.seg_slots = split.seg_slots;
+    a.c = LOG2E / o.temperature;
+    a.temperature = o.temperature;
+    a.ds = o;
+    GradArgs g{};
+    g.x = a.x;
+    g.dx = static_cast<char*>(o.dx);
+    g.x_pitch = o.x_pitch;
+    g.dx_pitch = o.dx_pitch;
+    g.cols = o.cols;
+    g.segs = grad_segs(o.cols);
+    g.c = a.c;
+    g.ds = o;
+    with_split_scratch(ctx, s, [&](void* scratch) {
+        const uint64_t per_row = sizeof(RowInfo) + (split.segs == 1 ? 0 : split.segs * sizeof(Part));
+        batches(o.rows, std::max(split.segs, g.segs), split_most(split.segs, per_row), [&](uint32_t r, uint32_t n) {
+            a.row0 = g.row0 = r;
+            a.tickets = reinterpret_cast<uint32_t*>(static_cast<char*>(scratch) + SPLIT_PARTIAL_MAX);
+            a.parts = static_cast<Part*>(scratch);
+            RowInfo* info = reinterpret_cast<RowInfo*>(a.parts + (split.segs == 1 ? 0 : static_cast<uint64_t>(n) * split.segs));
+            a.info = o.dx != nullptr ? info : nullptr;
+            g.info = info;
+            launch_pass<DT, false, false, true>(ctx, s, a, n);
+            if (o.dx != nullptr && o.cols > 0) launch_grad<DT, TEACHER>(ctx, s, g, n);
+        });
+    });
+}
+
+}  // namespace
+
+void launch_token_logprobs(lg_ctx* ctx, hipStream_t s, const LogprobArgs& a) {
+    a.dtype == LG_DTYPE_F32   ? logprobs_of<LG_DTYPE_F32>(ctx, s, a)
+    : a.dtype == LG_DTYPE_F16 ? logprobs_of<LG_DTYPE_F16>(ctx, s, a)
+                              : logprobs_of<LG_DTYPE_BF16>(ctx, s, a);
+}
+
+void launch_token_logprobs_backward(lg_ctx* ctx, hipStream_t s, const LogprobBackArgs& a) {
+    a.dtype == LG_DTYPE_F32   ? back_of<LG_DTYPE_F32>(ctx, s, a)
+    : a.dtype == LG_DTYPE_F16 ? back_of<LG_DTYPE_F16>(ctx, s, a)
+                              : back_of<LG_DTYPE_BF16>(ctx, s, a);
+}
+
+void launch_distill_grad(lg_ctx* ctx, hipStream_t s, const DistillArgs& a) {
+    a.dtype == LG_DTYPE_F32   ? distill_of<LG_DTYPE_F32>(ctx, s, a)
+    : a.dtype == LG_DTYPE_F16 ? distill_of<LG_DTYPE_F16>(ctx, s, a)
+                              : distill_of<LG_DTYPE_BF16>(ctx, s, a);
+}
+
+}  // namespace lg

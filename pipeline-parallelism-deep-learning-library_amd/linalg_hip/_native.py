@@ -20,6 +20,7 @@ LG_ELEM_F32, LG_ELEM_U32, LG_ELEM_I32, LG_ELEM_C32 = range(4)
 CORE_ERRORS = ["Ok", "Shape", "Dtype", "UnsupportedLayout", "UnsupportedDevice", "Alias",
                "Transport", "Wire", "Schedule"]
 LG_DTYPE_F32, LG_DTYPE_F16, LG_DTYPE_BF16 = 1, 2, 3
+LG_DTYPE_E4M3, LG_DTYPE_E8M0, LG_DTYPE_I32 = 16, 17, 18  # lg_head_dtype
 LG_WIRE_HEADER_MAX = 48
 PLAN_KINDS = ["empty", "zero", "scale", "tiled", "split", "general", "dot"]
 PLAN_KERNELS = ["none", "tile", "small", "wave", "dot", "outer", "direct", "pipelined", "streamk"]
@@ -98,6 +99,11 @@ SIGNATURES = {
     "lg_backend_convert": (i32, [vp, vp, TP, TP]),
     "lg_backend_download_into": (i32, [vp, vp, TP, vp, u64]),
     "lg_backend_upload_into": (i32, [vp, vp, vp, u64, TP]),
+    "lg_backend_quantize_blocks": (i32, [vp, vp, TP, TP, TP]),
+    "lg_backend_gemm_blocks": (i32, [vp, vp, TP, TP, TP, TP, TP, F, F]),
+    "lg_backend_token_logprobs": (i32, [vp, vp, TP, TP, F, TP, TP, TP, TP, TP]),
+    "lg_backend_token_logprobs_backward": (i32, [vp, vp, TP, TP, F, TP, TP, TP, TP, TP]),
+    "lg_backend_distill_grad": (i32, [vp, vp, TP, TP, TP, TP, F, i32, TP, TP]),
     "lg_wire_write_header": (i32, [u32, ctypes.POINTER(u64), u32, vp, ctypes.POINTER(u64)]),
     "lg_wire_parse_header": (i32, [vp, u64, ctypes.POINTER(u32), ctypes.POINTER(u64),
                                    ctypes.POINTER(u32), ctypes.POINTER(u64)]),

@@ -22,13 +22,19 @@ from .abi import Buffer, Context, NoDevice, alloc_shared
 
 
 class DType(enum.IntEnum):
-    """Wire tags of crates/core/src/lib.rs:10-32."""
+    """Wire tags of crates/core/src/lib.rs:10-32, and the element types that a head's operators
+    have beside them (no wire tags): OCP e4m3, e8m0 scales (2^(byte - 127)) and ids."""
     F32 = N.LG_DTYPE_F32
     F16 = N.LG_DTYPE_F16
     BF16 = N.LG_DTYPE_BF16
+    E4M3 = N.LG_DTYPE_E4M3
+    E8M0 = N.LG_DTYPE_E8M0
+    I32 = N.LG_DTYPE_I32
 
     def size_of(self) -> int:
-        return 4 if self is DType.F32 else 2
+        if self in (DType.F32, DType.I32):
+            return 4
+        return 2 if self in (DType.F16, DType.BF16) else 1
 
 
 class BackendError(Exception):
@@ -104,7 +110,7 @@ def transpose_matrix(t: Tensor) -> Tensor:
 
 
 def _refs(*tensors):
-    return [ctypes.byref(t.to_c()) for t in tensors]
+    return [None if t is None else ctypes.byref(t.to_c()) for t in tensors]
 
 
 def gemm_checks(a: Tensor, b: Tensor, c: Tensor, alpha: float, beta: float) -> None:
@@ -123,6 +129,39 @@ def op_checks(op: str, *args) -> None:
     if op == "mse_grad":
         scalars = [ctypes.byref(ctypes.c_float(0.0))]
     _raise(fn(None, None, *_refs(*tensors), *scalars))
+
+
+# A head's operators: their arguments in the entry points' order, "t" a tensor (or None where the
+# header allows it), "f" a float, "i" an int.
+_HEAD_OPS = {
+    "quantize_blocks": "ttt",
+    "gemm_blocks": "tttttff",
+    "token_logprobs": "ttfttttt",
+    "token_logprobs_backward": "ttfttttt",
+    "distill_grad": "ttttfitt",
+}
+
+
+def _head_args(op: str, args) -> list:
+    kinds = _HEAD_OPS[op]
+    if len(args) != len(kinds):
+        raise TypeError(f"{op} takes {len(kinds)} arguments, not {len(args)}")
+    return [_refs(a)[0] if k == "t" else float(a) if k == "f" else int(a) for k, a in zip(kinds, args)]
+
+
+def head_checks(op: str, *args) -> None:
+    """The checks of a head's operator ("quantize_blocks", "gemm_blocks", "token_logprobs",
+    "token_logprobs_backward" or "distill_grad") with no context: raises the first that fails, or
+    `UnsupportedDevice` ("null context") when all pass. Host only."""
+    _raise(getattr(N.lib(), f"lg_backend_{op}")(None, None, *_head_args(op, args)))
+
+
+def scales_shape(shape: Sequence[int], block_rows: int) -> List[int]:
+    """The shape of the scales of an [R, C] matrix: one for each 128 columns and `block_rows` (1 or
+    128) rows."""
+    if len(shape) != 2 or block_rows not in (1, 128):
+        raise BackendError("Shape", "scales need a rank-2 shape and blocks of 1 or 128 rows")
+    return [-(-shape[0] // block_rows), -(-shape[1] // 128)]
 
 
 def _nbytes(dtype: DType, shape: Sequence[int]) -> int:
@@ -244,6 +283,46 @@ class HipBackend:
     def convert(self, x: Tensor, y: Tensor) -> None:
         """`Backend::convert` (crates/core/src/lib.rs:229-236): F32 <-> BF16."""
         self._op("convert", *_refs(x, y))
+
+    def _head(self, op: str, *args) -> None:
+        self._op(op, *_head_args(op, args))
+
+    def quantize_blocks(self, x: Tensor, q: Tensor, scales: Tensor) -> None:
+        """q (E4M3), scales (F32 or E8M0) = x [R, C] with a scale for each 128 columns and each
+        row, or each 128 rows, as `scales_shape` says; x may be a `transpose_matrix` view."""
+        self._head("quantize_blocks", x, q, scales)
+
+    def gemm_blocks(self, a: Tensor, a_scales: Tensor, b: Tensor, b_scales: Tensor, c: Tensor,
+                    alpha: float = 1.0, beta: float = 0.0) -> None:
+        """c = alpha * A.B + beta * c of quantized operands; b is the `transpose_matrix` view of
+        the [N, K] matrix whose scales are `b_scales`."""
+        self._head("gemm_blocks", a, a_scales, b, b_scales, c, alpha, beta)
+
+    def token_logprobs(self, logits: Tensor, tokens: Optional[Tensor] = None,
+                       temperature: float = 1.0, logprobs: Optional[Tensor] = None,
+                       entropy: Optional[Tensor] = None, stats: Optional[Tensor] = None,
+                       top_logprobs: Optional[Tensor] = None,
+                       top_ids: Optional[Tensor] = None) -> None:
+        """Log probabilities of `tokens`, entropy, the gradient's statistics and the likeliest
+        alternatives of each row of logits, whichever outputs are given."""
+        self._head("token_logprobs", logits, tokens, temperature, logprobs, entropy, stats,
+                   top_logprobs, top_ids)
+
+    def token_logprobs_backward(self, logits: Tensor, tokens: Tensor, temperature: float,
+                                stats: Tensor, entropy: Optional[Tensor], dlogprobs: Tensor,
+                                dentropy: Optional[Tensor], dlogits: Tensor) -> None:
+        """dlogits from the gradients of log probabilities and (or None) of entropy; dlogits may be
+        logits."""
+        self._head("token_logprobs_backward", logits, tokens, temperature, stats, entropy,
+                   dlogprobs, dentropy, dlogits)
+
+    def distill_grad(self, logits: Tensor, teacher_ids: Tensor, teacher_logprobs: Tensor,
+                     weights: Optional[Tensor], temperature: float, normalize: bool,
+                     losses: Tensor, dlogits: Optional[Tensor]) -> None:
+        """Each row's loss against a teacher's likeliest alternatives and (or None) its gradient;
+        dlogits may be logits."""
+        self._head("distill_grad", logits, teacher_ids, teacher_logprobs, weights, temperature,
+                   bool(normalize), losses, dlogits)
 
     def sync(self) -> None:
         try:
