@@ -174,6 +174,219 @@ __global__ __launch_bounds__(THREADS) void gemm_blocks_any(GemmBlocksArgs g, uin
     }
 }
 
+// The same product of operands that allow 16-byte copies (bases, pitches and K in whole 16 bytes): a
+// TM x TN tile of C by WM x WN waves, slices of 128 columns copied from memory straight into LDS
+// (global_load_lds_dwordx4, [row][128] with the places of gemm_blocks_any) while the slice before is
+// multiplied. A slice's scales pass through registers into LDS beside it, one a thread.
+// FAST multiplies on v_mfma_f32_16x16x128_f8f6f4, one instruction to a block of 16x16 outputs, at the
+// precision above; e8m0 scales are then the instruction's own operands.
+__device__ inline void copy_sixteen(const uint8_t* src, uint8_t* lds) { __builtin_amdgcn_global_load_lds(src, lds, 16, 0, 0); }
+
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+
+template <bool FAST>
+struct Operand {
+    typedef Fragment T;
+};
+template <>
+struct Operand<true> {
+    struct T {
+        i32x8 v;
+        __device__ inline T() {}
+        __device__ inline T(u32x4 lo, u32x4 hi) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                v[i] = static_cast<int>(lo[i]);
+                v[i + 4] = static_cast<int>(hi[i]);
+            }
+        }
+    };
+};
+
+// Workgroup `id` of `count` to a tile: neighbouring ids go to the eight XCDs in turn, so each XCD takes one
+// run of tiles, and runs walk bands of eight tiles along M, whose operands its L2 then holds.
+__device__ inline void tile_of(uint32_t id, uint32_t tiles_m, uint32_t tiles_n, uint32_t* tm, uint32_t* tn) {
+    constexpr uint32_t XCDS = 8, BAND = 8;
+    const uint32_t count = tiles_m * tiles_n, per = count / XCDS, left = count % XCDS, xcd = id % XCDS;
+    const uint32_t t = xcd * per + min(xcd, left) + id / XCDS;
+    const uint32_t band = t / (BAND * tiles_n), first = band * BAND, high = min(BAND, tiles_m - first), in = t - first * tiles_n;
+    *tm = first + in % high;
+    *tn = in / high;
+}
+
+template <uint32_t OUT, bool FAST, bool E8M0, bool BROWS, int TM, int TN, int WM, int WN>
+__global__ __launch_bounds__(WM* WN * 64) void gemm_blocks_tile(GemmBlocksArgs g, uint32_t tiles_m, uint32_t tiles_n) {
+    constexpr int WAVES = WM * WN, T = WAVES * 64, FM = TM / WM / 16, FN = TN / WN / 16;
+    constexpr int STAGE = (TM + TN) * 128, COPIES = STAGE / 16 / T;  // copies a thread; A's rows first
+    constexpr bool HARDWARE = FAST && E8M0;
+    static_assert(BROWS || (TN / WN) % 128 == 0 || 128 % (TN / WN) == 0, "a wave's columns share their scale");
+    __shared__ __attribute__((aligned(16))) uint8_t stages[2][STAGE];
+    __shared__ __attribute__((aligned(16))) float scales[2][TM + TN];  // or e8m0 codes
+    const uint32_t tid = threadIdx.x, lane = tid % 64, wave = tid / 64;
+    uint32_t tm, tn;
+    tile_of(blockIdx.x, tiles_m, tiles_n, &tm, &tn);
+    const uint32_t m0 = tm * TM, n0 = tn * TN, wm = (wave % WM) * (TM / WM), wn = (wave / WM) * (TN / WN);
+    const uint32_t blocks = (g.k + BLOCK_K - 1) / BLOCK_K;
+    const uint8_t* pa = g.a + static_cast<int64_t>(m0) * g.a_pitch;
+    const uint8_t* pb = g.b + static_cast<int64_t>(n0) * g.b_pitch;
+    // Copy i of a wave: 1 KB of a stage, eight rows. Rows past the operand's last one repeat it.
+    static_assert(TM % (WAVES * 8) == 0 && TN % (WAVES * 8) == 0, "a copy is of one operand");
+    uint32_t offset[COPIES];
+#pragma unroll
+    for (int i = 0; i < COPIES; ++i) {
+        const uint32_t r = (i * WAVES + wave) * 8 + lane / 8, chunk = (lane % 8) ^ (r & 7);
+        const bool of_a = i * WAVES * 8 < TM;
+        const uint32_t row = of_a ? min(r, g.m - 1 - m0) : min(r - TM, g.n - 1 - n0);
+        offset[i] = row * static_cast<uint32_t>(of_a ? g.a_pitch : g.b_pitch) + chunk * 16;
+    }
+    auto copy = [&](uint32_t kb) {
+        const uint32_t left = g.k - kb * BLOCK_K;
+        uint8_t* stage = stages[kb % 2] + wave * 1024;
+        const uint8_t* a = pa + kb * BLOCK_K;
+        const uint8_t* b = pb + kb * BLOCK_K;
+        if (left >= BLOCK_K) {
+#pragma unroll
+            for (int i = 0; i < COPIES; ++i) copy_sixteen((i * WAVES * 8 < TM ? a : b) + offset[i], stage + i * WAVES * 1024);
+        } else {
+            const uint32_t lane_chunk = ((lane % 8) ^ (lane / 8)) * 16;  // of every copy: eight rows at a time
+#pragma unroll
+            for (int i = 0; i < COPIES; ++i) {
+                if (lane_chunk < left) {
+                    copy_sixteen((i * WAVES * 8 < TM ? a : b) + offset[i], stage + i * WAVES * 1024);
+                } else {
+                    *reinterpret_cast<u32x4*>(stage + i * WAVES * 1024 + lane * 16) = u32x4{0, 0, 0, 0};
+                }
+            }
+        }
+    };
+    // Thread t holds the scale of row t of the tile's operands (A's rows first) in the block to come.
+    constexpr int SCALES = (TM + TN + T - 1) / T;
+    float next[SCALES];
+    auto load_scales = [&](uint32_t kb) {
+#pragma unroll
+        for (int i = 0; i < SCALES; ++i) {
+            const uint32_t r = tid + i * T;
+            if (r >= TM + TN) break;
+            const bool of_a = r < TM;
+            const uint32_t row = of_a ? min(m0 + r, g.m - 1) : min(n0 + r - TM, g.n - 1);
+            const uint32_t block = of_a ? g.a_block : g.b_block;
+            const int64_t at = static_cast<int64_t>(block == 1 ? row : row / BLOCK_K) * (of_a ? g.sa_pitch : g.sb_pitch) + kb;
+            const void* p = of_a ? g.sa : g.sb;
+            if constexpr (HARDWARE) {
+                next[i] = __uint_as_float(static_cast<const uint8_t*>(p)[at]);
+            } else if constexpr (E8M0) {
+                next[i] = e8m0_value(static_cast<const uint8_t*>(p)[at]);
+            } else {
+                next[i] = static_cast<const float*>(p)[at];
+            }
+        }
+    };
+    f32x4 acc[FN][FM];
+#pragma unroll
+    for (int i = 0; i < FN; ++i) {
+#pragma unroll
+        for (int j = 0; j < FM; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    typedef typename Operand<FAST>::T Frag;
+    if (blocks > 0) {
+        load_scales(0);
+        copy(0);
+    }
+    for (uint32_t kb = 0; kb < blocks; ++kb) {
+        const uint8_t* stage = stages[kb % 2];
+        float* sc = scales[kb % 2];
+        __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): this wave's copies and scales have landed
+#pragma unroll
+        for (int i = 0; i < SCALES; ++i) {
+            if (tid + i * T < TM + TN) sc[tid + i * T] = next[i];
+        }
+        __syncthreads();
+        if (kb + 1 < blocks) {
+            load_scales(kb + 1);
+            copy(kb + 1);
+        }
+        auto fragment = [&](uint32_t r) {
+            const u32x4 lo = *reinterpret_cast<const u32x4*>(stage + r * 128 + ((lane / 16) ^ (r & 7)) * 16);
+            const u32x4 hi = *reinterpret_cast<const u32x4*>(stage + r * 128 + ((lane / 16 + 4) ^ (r & 7)) * 16);
+            return Frag(lo, hi);
+        };
+        Frag fa[FM];
+        float sa[FM];
+#pragma unroll
+        for (int j = 0; j < FM; ++j) {
+            fa[j] = fragment(wm + 16 * j + lane % 16);
+            sa[j] = sc[wm + 16 * j + lane % 16];
+        }
+        if constexpr (!BROWS && !HARDWARE) {
+            const float sb = sc[TM + wn];
+#pragma unroll
+            for (int j = 0; j < FM; ++j) sa[j] = sa[j] * sb;
+        }
+        // Row i of fragments: the next one's reads go first, and a product joins its sum LATE products later.
+        constexpr int LATE = 2, RING = 4;
+        Frag fb[2];
+        f32x4 sb[2], p[RING];
+        auto read_b = [&](int i) {
+            fb[i % 2] = fragment(TM + wn + 16 * i + lane % 16);
+            if constexpr (HARDWARE) {
+                sb[i % 2][0] = sc[TM + wn + 16 * i + lane % 16];
+            } else if constexpr (BROWS) {
+                sb[i % 2] = *reinterpret_cast<const f32x4*>(sc + TM + wn + 16 * i + (lane / 16) * 4);
+            }
+        };
+        auto join = [&](int t) {
+            const int i = t / FM, j = t % FM;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[i][j][e] = __builtin_fmaf(BROWS ? sa[j] * sb[i % 2][e] : sa[j], p[t % RING][e], acc[i][j][e]);
+        };
+        read_b(0);
+#pragma unroll
+        for (int i = 0; i < FN; ++i) {
+            if constexpr (!BROWS || HARDWARE) {
+                if (i + 1 < FN) read_b(i + 1);
+            }
+#pragma unroll
+            for (int j = 0; j < FM; ++j) {
+                const int t = i * FM + j;
+                if constexpr (HARDWARE) {
+                    acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fb[i % 2].v, fa[j].v, acc[i][j], 0, 0, 0, static_cast<int>(__float_as_uint(sb[i % 2][0])), 0,
+                                                                                 static_cast<int>(__float_as_uint(sa[j])));
+                } else {
+                    if constexpr (FAST) {
+                        p[t % RING] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fb[i % 2].v, fa[j].v, f32x4{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0, 0, 0, 0);
+                    } else {
+                        p[t % RING] = block_product(fb[i % 2], fa[j]);
+                    }
+                    if (t >= LATE) join(t - LATE);
+                }
+                if (BROWS && !HARDWARE && j == LATE - 1 && i + 1 < FN) read_b(i + 1);  // the row before has joined
+            }
+        }
+        if constexpr (!HARDWARE) {
+#pragma unroll
+            for (int t = FM * FN - LATE; t < FM * FN; ++t) join(t);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < FN; ++i) {
+#pragma unroll
+        for (int j = 0; j < FM; ++j) store_four<OUT>(g, m0 + wm + 16 * j + lane % 16, n0 + wn + 16 * i + (lane / 16) * 4, acc[i][j]);
+    }
+}
+
+template <uint32_t OUT, bool FAST, bool E8M0, bool BROWS, int TM, int TN, int WM, int WN>
+void launch_tile(lg_ctx* ctx, hipStream_t s, const GemmBlocksArgs& g) {
+    const uint32_t tm = (g.m + TM - 1) / TM, tn = (g.n + TN - 1) / TN;
+    hipLaunchKernelGGL((gemm_blocks_tile<OUT, FAST, E8M0, BROWS, TM, TN, WM, WN>), dim3(tm * tn), dim3(WM * WN * 64), 0, s, g, tm, tn);
+    launched(ctx, FAST ? "gemm_blocks_fp8" : "gemm_blocks_bf16");
+}
+
+bool copies_fit(const GemmBlocksArgs& g) {
+    const uint64_t all = reinterpret_cast<uintptr_t>(g.a) | reinterpret_cast<uintptr_t>(g.b) | static_cast<uint64_t>(g.a_pitch) |
+                         static_cast<uint64_t>(g.b_pitch) | g.k;
+    return all % 16 == 0 && g.a_pitch < (1 << 23) && g.b_pitch < (1 << 23);
+}
+
 template <uint32_t OUT, bool E8M0, int BA, int BB>
 void launch_of(lg_ctx* ctx, hipStream_t s, const GemmBlocksArgs& g) {
     const uint32_t tm = (g.m + TILE - 1) / TILE, tn = (g.n + TILE - 1) / TILE;
@@ -183,7 +396,25 @@ void launch_of(lg_ctx* ctx, hipStream_t s, const GemmBlocksArgs& g) {
 }
 
 template <uint32_t OUT, bool E8M0>
+bool launch_tiles(lg_ctx* ctx, hipStream_t s, const GemmBlocksArgs& g) {
+    if (!copies_fit(g) || g.m < 64 || g.n < 64) return false;
+    if (OUT != LG_DTYPE_F32 && g.k >= 512) {
+        if (g.b_block == 1) {
+            launch_tile<OUT, true, E8M0, true, 256, 256, 4, 2>(ctx, s, g);
+        } else {
+            launch_tile<OUT, true, E8M0, false, 256, 256, 4, 2>(ctx, s, g);
+        }
+    } else if (g.b_block == 1) {
+        launch_tile<OUT, false, E8M0, true, 128, 128, 2, 2>(ctx, s, g);
+    } else {
+        launch_tile<OUT, false, E8M0, false, 128, 128, 2, 2>(ctx, s, g);
+    }
+    return true;
+}
+
+template <uint32_t OUT, bool E8M0>
 void launch_blocks(lg_ctx* ctx, hipStream_t s, const GemmBlocksArgs& g) {
+    if (launch_tiles<OUT, E8M0>(ctx, s, g)) return;
     if (g.a_block == 1 && g.b_block == 1) {
         launch_of<OUT, E8M0, 1, 1>(ctx, s, g);
     } else if (g.a_block == 1) {
