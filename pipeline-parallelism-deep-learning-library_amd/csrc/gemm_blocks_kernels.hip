@@ -21,10 +21,10 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
 constexpr int THREADS = 256;
 
-// Eight e4m3 elements as bf16, which holds each of them.
-__device__ inline bf16x8 to_bf16(uint32_t lo, uint32_t hi) {
-    const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, false), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, true);
-    const bf16x2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, false), d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, true);
+// Eight e4m3 elements times s, a power of two, as bf16, which holds each of them.
+__device__ inline bf16x8 to_bf16(uint32_t lo, uint32_t hi, float s = 1.0f) {
+    const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, s, false), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, s, true);
+    const bf16x2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, s, false), d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, s, true);
     return bf16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
@@ -32,12 +32,11 @@ __device__ inline bf16x8 to_bf16(uint32_t lo, uint32_t hi) {
 struct Fragment {
     bf16x8 v[4];
     __device__ inline Fragment() {}
-    __device__ inline Fragment(u32x4 lo, u32x4 hi) : v{to_bf16(lo[0], lo[1]), to_bf16(lo[2], lo[3]), to_bf16(hi[0], hi[1]), to_bf16(hi[2], hi[3])} {}
+    __device__ inline Fragment(u32x4 lo, u32x4 hi, float s = 1.0f) : v{to_bf16(lo[0], lo[1], s), to_bf16(lo[2], lo[3], s), to_bf16(hi[0], hi[1], s), to_bf16(hi[2], hi[3], s)} {}
 };
 
 // A block's sums for 16x16 outputs.
-__device__ inline f32x4 block_product(const Fragment& b, const Fragment& a) {
-    f32x4 p = {0.0f, 0.0f, 0.0f, 0.0f};
+__device__ inline f32x4 block_product(const Fragment& b, const Fragment& a, f32x4 p = f32x4{0.0f, 0.0f, 0.0f, 0.0f}) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) p = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b.v[i], a.v[i], p, 0, 0, 0);
     return p;
@@ -174,12 +173,20 @@ __global__ __launch_bounds__(THREADS) void gemm_blocks_any(GemmBlocksArgs g, uin
     }
 }
 
-// The same product of operands that allow 16-byte copies (bases, pitches and K in whole 16 bytes): a
+// The product of operands that allow 16-byte copies (bases, pitches and K in whole 16 bytes): a
 // TM x TN tile of C by WM x WN waves, slices of 128 columns copied from memory straight into LDS
 // (global_load_lds_dwordx4, [row][128] with the places of gemm_blocks_any) while the slice before is
-// multiplied. A slice's scales pass through registers into LDS beside it, one a thread.
+// multiplied: four copies go out with each of the first rows of fragments, one row of B's fragments
+// is read ahead, and a product joins its sum two products later, so that neither LDS nor the multiply-adds
+// keep the matrix cores waiting. A slice's scales pass through registers into LDS beside it, one a thread.
 // FAST multiplies on v_mfma_f32_16x16x128_f8f6f4, one instruction to a block of 16x16 outputs, at the
-// precision above; e8m0 scales are then the instruction's own operands.
+// precision above; else in bf16. e8m0 scales cost nothing: the fp8 instruction takes them as operands, and the
+// conversion to bf16 applies them.
+// Bound by the issue of LDS reads, multiply-adds and matrix instructions of two waves a SIMD. Measured: 4096x65536x4096
+// into bf16, f32 scales on 256x256 tiles of eight waves, 1060 us (2080 TFLOP/s; a library product with one
+// scale 840 us), e8m0 990 us; with rows of C stored by lanes as they hold them 1190 us, with bands of eight tiles
+// 1070 us. 8192x8192x4096 into f32 on 128x128 tiles of four waves, two workgroups a compute unit: 513 us
+// (1070 TFLOP/s), on 256x128 tiles 517 us; 8192x2048x4096 with e8m0 scales 125 us, multiplied in afterwards 155 us.
 __device__ inline void copy_sixteen(const uint8_t* src, uint8_t* lds) { __builtin_amdgcn_global_load_lds(src, lds, 16, 0, 0); }
 
 typedef int i32x8 __attribute__((ext_vector_type(8)));
@@ -193,7 +200,7 @@ struct Operand<true> {
     struct T {
         i32x8 v;
         __device__ inline T() {}
-        __device__ inline T(u32x4 lo, u32x4 hi) {
+        __device__ inline T(u32x4 lo, u32x4 hi, float = 1.0f) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 v[i] = static_cast<int>(lo[i]);
@@ -204,9 +211,9 @@ struct Operand<true> {
 };
 
 // Workgroup `id` of `count` to a tile: neighbouring ids go to the eight XCDs in turn, so each XCD takes one
-// run of tiles, and runs walk bands of eight tiles along M, whose operands its L2 then holds.
+// run of tiles, and runs walk bands of four tiles along M, whose operands its L2 then holds.
 __device__ inline void tile_of(uint32_t id, uint32_t tiles_m, uint32_t tiles_n, uint32_t* tm, uint32_t* tn) {
-    constexpr uint32_t XCDS = 8, BAND = 8;
+        constexpr uint32_t XCDS = 8, BAND = 4;
     const uint32_t count = tiles_m * tiles_n, per = count / XCDS, left = count % XCDS, xcd = id % XCDS;
     const uint32_t t = xcd * per + min(xcd, left) + id / XCDS;
     const uint32_t band = t / (BAND * tiles_n), first = band * BAND, high = min(BAND, tiles_m - first), in = t - first * tiles_n;
@@ -215,14 +222,15 @@ __device__ inline void tile_of(uint32_t id, uint32_t tiles_m, uint32_t tiles_n, 
 }
 
 template <uint32_t OUT, bool FAST, bool E8M0, bool BROWS, int TM, int TN, int WM, int WN>
-__global__ __launch_bounds__(WM* WN * 64) void gemm_blocks_tile(GemmBlocksArgs g, uint32_t tiles_m, uint32_t tiles_n) {
+__global__ __launch_bounds__(WM* WN * 64) __attribute__((amdgpu_waves_per_eu(2))) void gemm_blocks_tile(GemmBlocksArgs g, uint32_t tiles_m, uint32_t tiles_n) {
     constexpr int WAVES = WM * WN, T = WAVES * 64, FM = TM / WM / 16, FN = TN / WN / 16;
     constexpr int STAGE = (TM + TN) * 128, COPIES = STAGE / 16 / T;  // copies a thread; A's rows first
-    constexpr bool HARDWARE = FAST && E8M0;
+    constexpr int COPIES_A_ROW = 4;                                  // of fragments
+    constexpr bool FOLDED = E8M0;  // the operands carry their scales
     static_assert(BROWS || (TN / WN) % 128 == 0 || 128 % (TN / WN) == 0, "a wave's columns share their scale");
     __shared__ __attribute__((aligned(16))) uint8_t stages[2][STAGE];
     __shared__ __attribute__((aligned(16))) float scales[2][TM + TN];  // or e8m0 codes
-    const uint32_t tid = threadIdx.x, lane = tid % 64, wave = tid / 64;
+    const uint32_t tid = threadIdx.x, lane = tid % 64, wave = __builtin_amdgcn_readfirstlane(tid / 64);
     uint32_t tm, tn;
     tile_of(blockIdx.x, tiles_m, tiles_n, &tm, &tn);
     const uint32_t m0 = tm * TM, n0 = tn * TN, wm = (wave % WM) * (TM / WM), wn = (wave / WM) * (TN / WN);
@@ -239,25 +247,15 @@ __global__ __launch_bounds__(WM* WN * 64) void gemm_blocks_tile(GemmBlocksArgs g
         const uint32_t row = of_a ? min(r, g.m - 1 - m0) : min(r - TM, g.n - 1 - n0);
         offset[i] = row * static_cast<uint32_t>(of_a ? g.a_pitch : g.b_pitch) + chunk * 16;
     }
-    auto copy = [&](uint32_t kb) {
-        const uint32_t left = g.k - kb * BLOCK_K;
-        uint8_t* stage = stages[kb % 2] + wave * 1024;
-        const uint8_t* a = pa + kb * BLOCK_K;
-        const uint8_t* b = pb + kb * BLOCK_K;
-        if (left >= BLOCK_K) {
-#pragma unroll
-            for (int i = 0; i < COPIES; ++i) copy_sixteen((i * WAVES * 8 < TM ? a : b) + offset[i], stage + i * WAVES * 1024);
-        } else {
-            const uint32_t lane_chunk = ((lane % 8) ^ (lane / 8)) * 16;  // of every copy: eight rows at a time
-#pragma unroll
-            for (int i = 0; i < COPIES; ++i) {
-                if (lane_chunk < left) {
-                    copy_sixteen((i * WAVES * 8 < TM ? a : b) + offset[i], stage + i * WAVES * 1024);
-                } else {
-                    *reinterpret_cast<u32x4*>(stage + i * WAVES * 1024 + lane * 16) = u32x4{0, 0, 0, 0};
-                }
-            }
-        }
+    const uint32_t lane_chunk = ((lane % 8) ^ (lane / 8)) * 16;  // of every copy: eight rows at a time
+    auto copy = [&](const uint8_t* a, const uint8_t* b, uint32_t at, int i) {
+        copy_sixteen((i * WAVES * 8 < TM ? a : b) + offset[i], stages[at] + (i * WAVES + wave) * 1024);
+    };
+    // The start of slice kb of an operand. (The compiler would otherwise keep a 64-bit address for every copy.)
+    auto slice = [](const uint8_t* p, uint32_t kb) {
+        p += kb * BLOCK_K;
+        __asm__("" : "+s"(p));
+        return p;
     };
     // Thread t holds the scale of row t of the tile's operands (A's rows first) in the block to come.
     constexpr int SCALES = (TM + TN + T - 1) / T;
@@ -272,7 +270,7 @@ __global__ __launch_bounds__(WM* WN * 64) void gemm_blocks_tile(GemmBlocksArgs g
             const uint32_t block = of_a ? g.a_block : g.b_block;
             const int64_t at = static_cast<int64_t>(block == 1 ? row : row / BLOCK_K) * (of_a ? g.sa_pitch : g.sb_pitch) + kb;
             const void* p = of_a ? g.sa : g.sb;
-            if constexpr (HARDWARE) {
+            if constexpr (FAST && E8M0) {
                 next[i] = __uint_as_float(static_cast<const uint8_t*>(p)[at]);
             } else if constexpr (E8M0) {
                 next[i] = e8m0_value(static_cast<const uint8_t*>(p)[at]);
@@ -288,51 +286,30 @@ __global__ __launch_bounds__(WM* WN * 64) void gemm_blocks_tile(GemmBlocksArgs g
         for (int j = 0; j < FM; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     }
     typedef typename Operand<FAST>::T Frag;
-    if (blocks > 0) {
-        load_scales(0);
-        copy(0);
-    }
-    for (uint32_t kb = 0; kb < blocks; ++kb) {
-        const uint8_t* stage = stages[kb % 2];
-        float* sc = scales[kb % 2];
-        __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): this wave's copies and scales have landed
-#pragma unroll
-        for (int i = 0; i < SCALES; ++i) {
-            if (tid + i * T < TM + TN) sc[tid + i * T] = next[i];
-        }
-        __syncthreads();
-        if (kb + 1 < blocks) {
-            load_scales(kb + 1);
-            copy(kb + 1);
-        }
-        auto fragment = [&](uint32_t r) {
-            const u32x4 lo = *reinterpret_cast<const u32x4*>(stage + r * 128 + ((lane / 16) ^ (r & 7)) * 16);
-            const u32x4 hi = *reinterpret_cast<const u32x4*>(stage + r * 128 + ((lane / 16 + 4) ^ (r & 7)) * 16);
-            return Frag(lo, hi);
+    // A product joins its sum LATE products later.
+    constexpr int LATE = 2, RING = 4;
+    // A fragment's row is lane % 16 past a multiple of 16, so its two chunks' places are the lane's own.
+    const uint32_t near = (lane % 16) * 128 + ((lane / 16) ^ (lane & 7)) * 16;
+    // Multiplies the slice in stage `at`; `more`: and copies slice kb, a whole one, into the other meanwhile.
+    auto multiply = [&](uint32_t at, bool more, uint32_t kb) {
+        const uint8_t* rows_a = stages[at] + wm * 128;
+        const uint8_t* rows_b = stages[at] + (TM + wn) * 128;
+        const float* sc = scales[at];
+        auto fragment = [&](const uint8_t* rows, int i, float scale = 1.0f) {
+            const u32x4 lo = *reinterpret_cast<const u32x4*>(rows + near + i * 2048);
+            const u32x4 hi = *reinterpret_cast<const u32x4*>(rows + (near ^ 64) + i * 2048);
+            return Frag(lo, hi, scale);
         };
-        Frag fa[FM];
+        Frag fa[FM], fb[2];
         float sa[FM];
-#pragma unroll
-        for (int j = 0; j < FM; ++j) {
-            fa[j] = fragment(wm + 16 * j + lane % 16);
-            sa[j] = sc[wm + 16 * j + lane % 16];
-        }
-        if constexpr (!BROWS && !HARDWARE) {
-            const float sb = sc[TM + wn];
-#pragma unroll
-            for (int j = 0; j < FM; ++j) sa[j] = sa[j] * sb;
-        }
-        // Row i of fragments: the next one's reads go first, and a product joins its sum LATE products later.
-        constexpr int LATE = 2, RING = 4;
-        Frag fb[2];
         f32x4 sb[2], p[RING];
         auto read_b = [&](int i) {
-            fb[i % 2] = fragment(TM + wn + 16 * i + lane % 16);
-            if constexpr (HARDWARE) {
+            if constexpr (FOLDED) {
                 sb[i % 2][0] = sc[TM + wn + 16 * i + lane % 16];
             } else if constexpr (BROWS) {
                 sb[i % 2] = *reinterpret_cast<const f32x4*>(sc + TM + wn + 16 * i + (lane / 16) * 4);
             }
+            fb[i % 2] = fragment(rows_b, i, FOLDED ? sb[i % 2][0] : 1.0f);
         };
         auto join = [&](int t) {
             const int i = t / FM, j = t % FM;
@@ -341,14 +318,35 @@ __global__ __launch_bounds__(WM* WN * 64) void gemm_blocks_tile(GemmBlocksArgs g
         };
         read_b(0);
 #pragma unroll
+        for (int j = 0; j < FM; ++j) {
+            sa[j] = sc[wm + 16 * j + lane % 16];
+            fa[j] = fragment(rows_a, j, FOLDED ? sa[j] : 1.0f);
+        }
+        if constexpr (!BROWS && !FOLDED) {
+            const float b = sc[TM + wn];
+#pragma unroll
+            for (int j = 0; j < FM; ++j) sa[j] = sa[j] * b;
+        }
+        if (more) load_scales(kb);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
         for (int i = 0; i < FN; ++i) {
-            if constexpr (!BROWS || HARDWARE) {
+            if constexpr (!BROWS || FOLDED) {
                 if (i + 1 < FN) read_b(i + 1);
+            }
+            if (more && i * COPIES_A_ROW < COPIES) {
+                const uint8_t *ca = slice(pa, kb), *cb = slice(pb, kb);
+#pragma unroll
+                for (int q = 0; q < COPIES_A_ROW; ++q) {
+                    if (i * COPIES_A_ROW + q < COPIES) copy(ca, cb, at ^ 1, i * COPIES_A_ROW + q);
+                }
             }
 #pragma unroll
             for (int j = 0; j < FM; ++j) {
                 const int t = i * FM + j;
-                if constexpr (HARDWARE) {
+                if constexpr (FOLDED && !FAST) {
+                    acc[i][j] = block_product(fb[i % 2], fa[j], acc[i][j]);
+                } else if constexpr (FOLDED) {
                     acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fb[i % 2].v, fa[j].v, acc[i][j], 0, 0, 0, static_cast<int>(__float_as_uint(sb[i % 2][0])), 0,
                                                                                  static_cast<int>(__float_as_uint(sa[j])));
                 } else {
@@ -359,18 +357,101 @@ __global__ __launch_bounds__(WM* WN * 64) void gemm_blocks_tile(GemmBlocksArgs g
                     }
                     if (t >= LATE) join(t - LATE);
                 }
-                if (BROWS && !HARDWARE && j == LATE - 1 && i + 1 < FN) read_b(i + 1);  // the row before has joined
+                if (BROWS && !FOLDED && j == LATE - 1 && i + 1 < FN) read_b(i + 1);  // the row before has joined
             }
+            if constexpr (!FAST) {
+#pragma unroll
+                for (int j = 0; j < 4 * FM; ++j) {
+                    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                    if (j < 2) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+                    __builtin_amdgcn_sched_group_barrier(0x002, 2, 0);
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < FM; ++j) {
+                    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                    if (j < 2) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+                    if (!FOLDED) __builtin_amdgcn_sched_group_barrier(0x002, 4, 0);
+                }
+            }
+            __builtin_amdgcn_sched_barrier(0);
         }
-        if constexpr (!HARDWARE) {
+        if constexpr (!FOLDED) {
 #pragma unroll
             for (int t = FM * FN - LATE; t < FM * FN; ++t) join(t);
         }
+    };
+    // The last slice, which may be of fewer than 128 columns, goes first, with zeros in the places past them.
+    if (blocks > 0) {
+        const uint32_t kb = blocks - 1;
+        load_scales(kb);
+#pragma unroll
+        for (int i = 0; i < COPIES; ++i) {
+            if (kb * BLOCK_K + lane_chunk < g.k) {
+                copy(slice(pa, kb), slice(pb, kb), 0, i);
+            } else {
+                *reinterpret_cast<u32x4*>(stages[0] + (i * WAVES + wave) * 1024 + lane * 16) = u32x4{0, 0, 0, 0};
+            }
+        }
     }
+    for (uint32_t s = 0; s < blocks; ++s) {
+        float* sc = scales[s % 2];
+        __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): this wave's copies and scales have landed
+#pragma unroll
+        for (int i = 0; i < SCALES; ++i) {
+            if (tid + i * T < TM + TN) sc[tid + i * T] = next[i];
+        }
+        __syncthreads();
+        multiply(s % 2, s + 1 < blocks, s);
+    }
+    if (g.beta != 0.0f) {
+#pragma unroll
+        for (int i = 0; i < FN; ++i) {
+#pragma unroll
+            for (int j = 0; j < FM; ++j) store_four<OUT>(g, m0 + wm + 16 * j + lane % 16, n0 + wn + 16 * i + (lane / 16) * 4, acc[i][j]);
+        }
+        return;
+    }
+    // A wave's outputs pass through its own part of the stages, so that rows leave as whole runs of 16 bytes a lane:
+    // [row][16-byte chunk], chunk c of row r at place c ^ (r % CHUNKS).
+    constexpr int ROW = TN / WN * static_cast<int>(elem_size<OUT>), CHUNKS = ROW / 16, PER = 16 / static_cast<int>(elem_size<OUT>);
+    static_assert((CHUNKS == 8 || CHUNKS == 16) && TM / WM * ROW * WAVES <= 2 * STAGE, "a wave's outputs fit its part of the stages");
+    __syncthreads();  // every wave is done with the stages
+    uint8_t* mine = &stages[0][0] + wave * (TM / WM * ROW);
 #pragma unroll
     for (int i = 0; i < FN; ++i) {
 #pragma unroll
-        for (int j = 0; j < FM; ++j) store_four<OUT>(g, m0 + wm + 16 * j + lane % 16, n0 + wn + 16 * i + (lane / 16) * 4, acc[i][j]);
+        for (int j = 0; j < FM; ++j) {
+            const uint32_t r = 16 * j + lane % 16, byte = (16 * i + (lane / 16) * 4) * elem_size<OUT>;
+            uint8_t* to = mine + r * ROW + (((byte / 16) ^ (r % CHUNKS)) * 16 + byte % 16);
+            const f32x4 v = acc[i][j] * g.alpha;
+            if constexpr (OUT == LG_DTYPE_F32) {
+                *reinterpret_cast<f32x4*>(to) = v;
+            } else {
+                *reinterpret_cast<u32x2*>(to) = u32x2{pack2<OUT>(v[0], v[1]), pack2<OUT>(v[2], v[3])};
+            }
+        }
+    }
+    // The wave's own writes only: no other wave reads them.
+    __builtin_amdgcn_wave_barrier();
+    const uint32_t c = lane % CHUNKS, n = n0 + wn + c * PER;
+#pragma unroll
+    for (int q = 0; q < TM / WM * CHUNKS / 64; ++q) {
+        const uint32_t r = q * (64 / CHUNKS) + lane / CHUNKS, m = m0 + wm + r;
+        const u32x4 v = *reinterpret_cast<const u32x4*>(mine + r * ROW + (c ^ (r % CHUNKS)) * 16);
+        if (m >= g.m || n >= g.n) continue;
+        char* to = static_cast<char*>(g.c) + (m * g.c_pitch + n) * elem_size<OUT>;
+        if (n + PER <= g.n) {
+            *reinterpret_cast<u32x4_any*>(to) = v;
+        } else {
+            for (uint32_t e = 0; n + e < g.n; ++e) {
+                if constexpr (OUT == LG_DTYPE_F32) {
+                    reinterpret_cast<uint32_t*>(to)[e] = v[e];
+                } else {
+                    reinterpret_cast<uint16_t*>(to)[e] = static_cast<uint16_t>(v[e / 2] >> (16 * (e % 2)));
+                }
+            }
+        }
     }
 }
 
@@ -398,13 +479,17 @@ void launch_of(lg_ctx* ctx, hipStream_t s, const GemmBlocksArgs& g) {
 template <uint32_t OUT, bool E8M0>
 bool launch_tiles(lg_ctx* ctx, hipStream_t s, const GemmBlocksArgs& g) {
     if (!copies_fit(g) || g.m < 64 || g.n < 64) return false;
-    if (OUT != LG_DTYPE_F32 && g.k >= 512) {
-        if (g.b_block == 1) {
-            launch_tile<OUT, true, E8M0, true, 256, 256, 4, 2>(ctx, s, g);
-        } else {
-            launch_tile<OUT, true, E8M0, false, 256, 256, 4, 2>(ctx, s, g);
+    if constexpr (OUT != LG_DTYPE_F32) {
+        if (g.k >= 512) {
+            if (g.b_block == 1) {
+                launch_tile<OUT, true, E8M0, true, 256, 256, 4, 2>(ctx, s, g);
+            } else {
+                launch_tile<OUT, true, E8M0, false, 256, 256, 4, 2>(ctx, s, g);
+            }
+            return true;
         }
-    } else if (g.b_block == 1) {
+    }
+    if (g.b_block == 1) {
         launch_tile<OUT, false, E8M0, true, 128, 128, 2, 2>(ctx, s, g);
     } else {
         launch_tile<OUT, false, E8M0, false, 128, 128, 2, 2>(ctx, s, g);
