@@ -43,7 +43,9 @@ SOURCES = [
     "backend_gemm16_kernels.hip",
     "head.cpp",
     "quantize_kernels.hip",
-    "gemm_blocks_kernels.hip",
+    "gemm_blocks_f32_kernels.hip",
+    "gemm_blocks_f16_kernels.hip",
+    "gemm_blocks_bf16_kernels.hip",
     "logits_kernels.hip",
 ]
 

@@ -1,0 +1,644 @@
+// gfx950 kernels of gemm_blocks: C = alpha * sum over blocks b of sa[m, b] sb[n, b] (A_b . B_b^T) + beta * C
+// of e4m3 operands with a scale for each 128 columns of K and each row, or each 128 rows.
+//
+// The fp8 matrix instructions align each eight neighbouring products to the largest of them and keep 2^-13 of
+// it (measured: 1.5e-5 of the norm for normal operands, 1.2e-5 of the sum of absolute products at K = 128).
+// Where that is not enough the kernels turn elements into bf16, which holds every e4m3 value, two to an instruction on
+// their way to the matrix cores, and multiply on v_mfma_f32_16x16x32_bf16: four of those are a block's sum for 16x16
+// outputs, exact products summed in f32 (7e-8 of the norm at K = 4096). The instructions' order of K is free
+// as long as both operands share it: a lane takes 32 bytes of one row of each operand (row lane % 16, the
+// quarter of the block goes by lane / 16) and eight of them per instruction. B's rows are the first operand and
+// A's the second, so a lane's four outputs are neighbours along N of one row of C. A block's sums start
+// at zero and join the f32 accumulator by a multiply-add with sa * sb; e8m0 scales are applied by the
+// conversion, or are the fp8 instruction's own operands.
+#pragma once
+
+#include "head_device.h"
+
+namespace lg {
+namespace {
+
+using namespace head_detail;
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+
+// Eight e4m3 elements times s, a power of two, as bf16, which holds each of them.
+__device__ inline bf16x8 to_bf16(uint32_t lo, uint32_t hi, float s = 1.0f) {
+    const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, s, false), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, s, true);
+    const bf16x2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, s, false), d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, s, true);
+    return bf16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+
+// A lane's part of a row in a block of 128: 32 elements.
+struct Fragment {
+    bf16x8 v[4];
+    __device__ inline Fragment() {}
+    __device__ inline Fragment(u32x4 lo, u32x4 hi, float s = 1.0f) : v{to_bf16(lo[0], lo[1], s), to_bf16(lo[2], lo[3], s), to_bf16(hi[0], hi[1], s), to_bf16(hi[2], hi[3], s)} {}
+};
+
+// A block's sums for 16x16 outputs.
+__device__ inline f32x4 block_product(const Fragment& b, const Fragment& a, f32x4 p = f32x4{0.0f, 0.0f, 0.0f, 0.0f}) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) p = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b.v[i], a.v[i], p, 0, 0, 0);
+    return p;
+}
+
+__device__ inline float e8m0_value(uint32_t code) {
+    // 2^-127, code 0, is subnormal.
+    return code == 255 ? __builtin_nanf("") : __uint_as_float(code == 0 ? 0x400000u : code << 23);
+}
+
+// Bytes k .. k + 15 of a row of length K at any address, zeros past its end.
+__device__ inline u32x4 load_sixteen(const uint8_t* row, uint32_t k, uint32_t K) {
+    if (k + 16 <= K) return *reinterpret_cast<const u32x4_any*>(row + k);
+    u32x4 v = {0, 0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        if (k + i < K) v[i / 4] |= static_cast<uint32_t>(row[k + i]) << (8 * (i % 4));
+    }
+    return v;
+}
+
+// Outputs (m, n .. n + 3), those inside C, from the sums of a lane.
+template <uint32_t OUT>
+__device__ inline void store_four(const GemmBlocksArgs& g, uint32_t m, uint32_t n, f32x4 acc) {
+    if (m >= g.m || n >= g.n) return;
+    char* p = static_cast<char*>(g.c) + (m * g.c_pitch + n) * elem_size<OUT>;
+    float v[4];
+    const uint32_t inside = min(g.n - n, 4u);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        v[e] = g.alpha * acc[e];
+        if (g.beta != 0.0f && static_cast<uint32_t>(e) < inside) v[e] = v[e] + g.beta * load_one<OUT>(p + e * elem_size<OUT>);
+    }
+    if (inside == 4) {
+        if constexpr (OUT == LG_DTYPE_F32) {
+            u32x4 o;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] = __float_as_uint(v[e]);
+            *reinterpret_cast<u32x4_any*>(p) = o;
+        } else {
+            *reinterpret_cast<u32x2_any*>(p) = u32x2{pack2<OUT>(v[0], v[1]), pack2<OUT>(v[2], v[3])};
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            if (static_cast<uint32_t>(e) < inside) store_one<OUT>(p + e * elem_size<OUT>, v[e]);
+        }
+    }
+}
+
+// A TM x TN tile of C by KG groups of WM x WN waves. Slices of 128 columns lie in LDS as [row][128] with 16-byte
+// chunk c of row r at place c ^ (r & 7), so that eight neighbouring rows' reads of one chunk touch every bank once,
+// two stages of KG slices each. DIRECT (bases, pitches and K in whole 16 bytes): copied from memory straight into LDS
+// (global_load_lds_dwordx4) while the stage before is multiplied; else through registers, any addresses. Four copies
+// go out with each of the first rows of fragments, one row of B's fragments is read ahead, and a product joins its sum
+// two products later, so that neither LDS nor the multiply-adds keep the matrix cores waiting. A slice's scales
+// pass through registers into LDS beside it. Groups take slices in turn and add their sums in LDS at the end: more
+// waves for outputs of few tiles.
+// FAST multiplies on v_mfma_f32_16x16x128_f8f6f4, one instruction to a block of 16x16 outputs, at the precision
+// above; else in bf16.
+// Bound by the issue of LDS reads, multiply-adds and matrix instructions of two waves a SIMD; of few tiles by the
+// latency of a stage. Measured: 4096x65536x4096 into bf16, f32 scales on 256x256 tiles of eight waves, 1060 us (2080
+// TFLOP/s; a library product with one scale 840 us), e8m0 990 us; with rows of C stored by lanes as they hold them 1190 us,
+// with bands of eight tiles 1070 us. 8192x8192x4096 into f32 on 128x128 tiles of four waves, two workgroups a compute
+// unit: 513 us (1070 TFLOP/s), on 256x128 tiles 517 us; 8192x2048x4096 with e8m0 scales 125 us, multiplied in afterwards
+// 155 us. 512x2048x4096 into f32 on 64x64 tiles of two groups 18 us, on 128x128 tiles 40 us. 77x4099x2011 into f32
+// through registers on 32x64 tiles of four groups 12.2 us, on 64x64 tiles of two 16 us, of one 20 us.
+__device__ inline void copy_sixteen(const uint8_t* src, uint8_t* lds) { __builtin_amdgcn_global_load_lds(src, lds, 16, 0, 0); }
+
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+
+template <bool FAST>
+struct Operand {
+    typedef Fragment T;
+};
+template <>
+struct Operand<true> {
+    struct T {
+        i32x8 v;
+        __device__ inline T() {}
+        __device__ inline T(u32x4 lo, u32x4 hi, float = 1.0f) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                v[i] = static_cast<int>(lo[i]);
+                v[i + 4] = static_cast<int>(hi[i]);
+            }
+        }
+    };
+};
+
+// Workgroup `id` of `count` to a tile: neighbouring ids go to the eight XCDs in turn, so each XCD takes one
+// run of tiles, and runs walk bands of four tiles along M, whose operands its L2 then holds.
+__device__ inline void tile_of(uint32_t id, uint32_t tiles_m, uint32_t tiles_n, uint32_t* tm, uint32_t* tn) {
+        constexpr uint32_t XCDS = 8, BAND = 4;
+    const uint32_t count = tiles_m * tiles_n, per = count / XCDS, left = count % XCDS, xcd = id % XCDS;
+    const uint32_t t = xcd * per + min(xcd, left) + id / XCDS;
+    const uint32_t band = t / (BAND * tiles_n), first = band * BAND, high = min(BAND, tiles_m - first), in = t - first * tiles_n;
+    *tm = first + in % high;
+    *tn = in / high;
+}
+
+template <uint32_t OUT, bool DIRECT, bool FAST, bool E8M0, bool BROWS, int TM, int TN, int WM, int WN, int KG>
+__global__ __launch_bounds__(WM* WN * KG * 64) __attribute__((amdgpu_waves_per_eu(WM * WN * KG > 8 ? WM * WN * KG / 4 : 2))) void gemm_blocks_tile(GemmBlocksArgs g, uint32_t tiles_m, uint32_t tiles_n) {
+    constexpr int WAVES = WM * WN * KG, T = WAVES * 64, FM = TM / WM / 16, FN = TN / WN / 16;
+    constexpr int SLICE = (TM + TN) * 128, STAGE = KG * SLICE, COPIES = STAGE / 16 / T;  // copies a thread; A's rows first
+    constexpr int COPIES_A_ROW = 4;                                  // of fragments
+    constexpr bool FOLDED = E8M0;  // the operands carry their scales
+    static_assert(BROWS || (TN / WN) % 128 == 0 || 128 % (TN / WN) == 0, "a wave's columns share their scale");
+    __shared__ __attribute__((aligned(16))) uint8_t stages[2][STAGE];
+    __shared__ __attribute__((aligned(16))) float scales[2][KG][TM + TN];  // or e8m0 codes
+    const uint32_t tid = threadIdx.x, lane = tid % 64, wave = __builtin_amdgcn_readfirstlane(tid / 64);
+    const uint32_t kg = wave / (WM * WN);  // the group's slices: kg, kg + KG ...
+    uint32_t tm, tn;
+    tile_of(blockIdx.x, tiles_m, tiles_n, &tm, &tn);
+    const uint32_t m0 = tm * TM, n0 = tn * TN, wm = (wave % WM) * (TM / WM), wn = (wave / WM % WN) * (TN / WN);
+    const uint32_t blocks = (g.k + BLOCK_K - 1) / BLOCK_K;
+    const uint8_t* pa = g.a + static_cast<int64_t>(m0) * g.a_pitch;
+    const uint8_t* pb = g.b + static_cast<int64_t>(n0) * g.b_pitch;
+    // Copy i of a wave: 1 KB of a stage, eight rows. Rows past the operand's last one repeat it.
+    // Groups of waves copy their own slices.
+    constexpr int GW = WM * WN;
+    const uint32_t gwave = wave % GW;
+    static_assert(TM % (GW * 8) == 0 && TN % (GW * 8) == 0, "a copy is of one operand");
+    uint32_t offset[COPIES];
+#pragma unroll
+    for (int i = 0; i < COPIES; ++i) {
+        const uint32_t r = (i * GW + gwave) * 8 + lane / 8, chunk = (lane % 8) ^ (r & 7);
+        const bool of_a = i * GW * 8 < TM;
+        const uint32_t row = of_a ? min(r, g.m - 1 - m0) : min(r - TM, g.n - 1 - n0);
+        offset[i] = row * static_cast<uint32_t>(of_a ? g.a_pitch : g.b_pitch) + chunk * 16;
+    }
+    u32x4 held[DIRECT ? 1 : COPIES];
+    const uint32_t lane_chunk = ((lane % 8) ^ (lane / 8)) * 16;  // of every copy: eight rows at a time
+    auto copy = [&](const uint8_t* a, const uint8_t* b, uint32_t at, int i) {
+        const uint8_t* from = (i * GW * 8 < TM ? a : b) + offset[i];
+        if constexpr (DIRECT) {
+            copy_sixteen(from, stages[at] + kg * SLICE + (i * GW + gwave) * 1024);
+        } else {
+            held[i] = *reinterpret_cast<const u32x4_any*>(from);
+        }
+    };
+    // The start of slice kb of an operand. (The compiler would otherwise keep a 64-bit address for every copy.)
+    auto slice = [](const uint8_t* p, uint32_t kb) {
+        p += kb * BLOCK_K;
+        __asm__("" : "+s"(p));
+        return p;
+    };
+    // Thread t holds the scale of row t of the tile's operands (A's rows first) in the block to come.
+    constexpr int SCALES = (TM + TN + GW * 64 - 1) / (GW * 64);
+    const uint32_t gtid = tid % (GW * 64);
+    float next[SCALES];
+    auto load_scales = [&](uint32_t kb) {
+#pragma unroll
+        for (int i = 0; i < SCALES; ++i) {
+            const uint32_t r = gtid + i * GW * 64;
+            if (r >= TM + TN) break;
+            const bool of_a = r < TM;
+            const uint32_t row = of_a ? min(m0 + r, g.m - 1) : min(n0 + r - TM, g.n - 1);
+            const uint32_t block = of_a ? g.a_block : g.b_block;
+            const int64_t at = static_cast<int64_t>(block == 1 ? row : row / BLOCK_K) * (of_a ? g.sa_pitch : g.sb_pitch) + kb;
+            const void* p = of_a ? g.sa : g.sb;
+            if constexpr (FAST && E8M0) {
+                next[i] = __uint_as_float(static_cast<const uint8_t*>(p)[at]);
+            } else if constexpr (E8M0) {
+                next[i] = e8m0_value(static_cast<const uint8_t*>(p)[at]);
+            } else {
+                next[i] = static_cast<const float*>(p)[at];
+            }
+        }
+    };
+    f32x4 acc[FN][FM];
+#pragma unroll
+    for (int i = 0; i < FN; ++i) {
+#pragma unroll
+        for (int j = 0; j < FM; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    typedef typename Operand<FAST>::T Frag;
+    // A product joins its sum LATE products later.
+    constexpr int LATE = 2, RING = 4;
+    // A fragment's row is lane % 16 past a multiple of 16, so its two chunks' places are the lane's own.
+    const uint32_t near = (lane % 16) * 128 + ((lane / 16) ^ (lane & 7)) * 16;
+    // Multiplies the slice in stage `at`; `more`: and copies slice kb, a whole one, into the other meanwhile.
+    auto multiply = [&](uint32_t at, bool more, uint32_t kb) {
+        const uint8_t* rows_a = stages[at] + kg * SLICE + wm * 128;
+        const uint8_t* rows_b = stages[at] + kg * SLICE + (TM + wn) * 128;
+        const float* sc = scales[at][kg];
+        auto fragment = [&](const uint8_t* rows, int i, float scale = 1.0f) {
+            const u32x4 lo = *reinterpret_cast<const u32x4*>(rows + near + i * 2048);
+            const u32x4 hi = *reinterpret_cast<const u32x4*>(rows + (near ^ 64) + i * 2048);
+            return Frag(lo, hi, scale);
+        };
+        Frag fa[FM], fb[2];
+        float sa[FM];
+        f32x4 sb[2], p[RING];
+        auto read_b = [&](int i) {
+            if constexpr (FOLDED) {
+                sb[i % 2][0] = sc[TM + wn + 16 * i + lane % 16];
+            } else if constexpr (BROWS) {
+                sb[i % 2] = *reinterpret_cast<const f32x4*>(sc + TM + wn + 16 * i + (lane / 16) * 4);
+            }
+            fb[i % 2] = fragment(rows_b, i, FOLDED ? sb[i % 2][0] : 1.0f);
+        };
+        auto join = [&](int t) {
+            const int i = t / FM, j = t % FM;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[i][j][e] = __builtin_fmaf(BROWS ? sa[j] * sb[i % 2][e] : sa[j], p[t % RING][e], acc[i][j][e]);
+        };
+        read_b(0);
+#pragma unroll
+        for (int j = 0; j < FM; ++j) {
+            sa[j] = sc[wm + 16 * j + lane % 16];
+            fa[j] = fragment(rows_a, j, FOLDED ? sa[j] : 1.0f);
+        }
+        if constexpr (!BROWS && !FOLDED) {
+            const float b = sc[TM + wn];
+#pragma unroll
+            for (int j = 0; j < FM; ++j) sa[j] = sa[j] * b;
+        }
+        if (more) load_scales(kb);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < FN; ++i) {
+            if constexpr (!BROWS || FOLDED) {
+                if (i + 1 < FN) read_b(i + 1);
+            }
+            if (more && i * COPIES_A_ROW < COPIES) {
+                const uint8_t *ca = slice(pa, kb), *cb = slice(pb, kb);
+#pragma unroll
+                for (int q = 0; q < COPIES_A_ROW; ++q) {
+                    if (i * COPIES_A_ROW + q < COPIES) copy(ca, cb, at ^ 1, i * COPIES_A_ROW + q);
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < FM; ++j) {
+                const int t = i * FM + j;
+                if constexpr (FOLDED && !FAST) {
+                    acc[i][j] = block_product(fb[i % 2], fa[j], acc[i][j]);
+                } else if constexpr (FOLDED) {
+                    acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fb[i % 2].v, fa[j].v, acc[i][j], 0, 0, 0, static_cast<int>(__float_as_uint(sb[i % 2][0])), 0,
+                                                                                 static_cast<int>(__float_as_uint(sa[j])));
+                } else {
+                    if constexpr (FAST) {
+                        p[t % RING] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fb[i % 2].v, fa[j].v, f32x4{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0, 0, 0, 0);
+                    } else {
+                        p[t % RING] = block_product(fb[i % 2], fa[j]);
+                    }
+                    if (t >= LATE) join(t - LATE);
+                }
+                if (BROWS && !FOLDED && j == LATE - 1 && i + 1 < FN) read_b(i + 1);  // the row before has joined
+            }
+            if constexpr (!FAST) {
+#pragma unroll
+                for (int j = 0; j < 4 * FM; ++j) {
+                    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                    if (j < 2) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+                    __builtin_amdgcn_sched_group_barrier(0x002, 2, 0);
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < FM; ++j) {
+                    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                    if (j < 2) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+                    if (!FOLDED) __builtin_amdgcn_sched_group_barrier(0x002, 4, 0);
+                }
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        if constexpr (!FOLDED) {
+#pragma unroll
+            for (int t = FM * FN - LATE; t < FM * FN; ++t) join(t);
+        }
+    };
+    // The last slice, which may be of fewer than 128 columns, goes first, with zeros in the places past them; then the
+    // others in order: turn q of group kg is slice q * KG + kg - 1.
+    const uint32_t turns = (blocks + KG - 1) / KG;
+    if (kg < blocks) {
+        const uint32_t kb = kg == 0 ? blocks - 1 : kg - 1;
+        load_scales(kb);
+#pragma unroll
+        for (int i = 0; i < COPIES; ++i) {
+            if constexpr (DIRECT) {
+                if (kb * BLOCK_K + lane_chunk < g.k) {
+                    copy(slice(pa, kb), slice(pb, kb), 0, i);
+                } else {
+                    *reinterpret_cast<u32x4*>(stages[0] + kg * SLICE + (i * GW + gwave) * 1024 + lane * 16) = u32x4{0, 0, 0, 0};
+                }
+            } else if ((kb + 1) * BLOCK_K <= g.k) {
+                copy(slice(pa, kb), slice(pb, kb), 0, i);
+            } else {
+                held[i] = load_sixteen((i * GW * 8 < TM ? pa : pb) + (offset[i] - lane_chunk), kb * BLOCK_K + lane_chunk, g.k);
+            }
+        }
+    }
+    for (uint32_t s = 0; s < turns; ++s) {
+        const bool live = s * KG + kg < blocks;
+        float* sc = scales[s % 2][kg];
+        if (live) {
+            if constexpr (DIRECT) {
+                __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): this wave's copies and scales have landed
+            } else {
+#pragma unroll
+                for (int i = 0; i < COPIES; ++i) *reinterpret_cast<u32x4*>(stages[s % 2] + kg * SLICE + (i * GW + gwave) * 1024 + lane * 16) = held[i];
+            }
+#pragma unroll
+            for (int i = 0; i < SCALES; ++i) {
+                if (gtid + i * GW * 64 < TM + TN) sc[gtid + i * GW * 64] = next[i];
+            }
+        }
+        __syncthreads();
+        if (live) multiply(s % 2, (s + 1) * KG + kg < blocks, (s + 1) * KG + kg - 1);
+    }
+    if constexpr (KG > 1) {
+        // The groups' sums meet in LDS, in their order.
+        constexpr int SUMS = FM * FN * 1024;  // bytes of a wave
+        static_assert((KG - 1) * GW * SUMS <= 2 * STAGE, "the groups' sums fit the stages");
+        uint8_t* sums = &stages[0][0];
+        __syncthreads();
+        if (kg > 0) {
+#pragma unroll
+            for (int i = 0; i < FN * FM; ++i) *reinterpret_cast<f32x4*>(sums + ((kg - 1) * GW + gwave) * SUMS + i * 1024 + lane * 16) = acc[i / FM][i % FM];
+        }
+        __syncthreads();
+        if (kg > 0) return;
+#pragma unroll
+        for (int o = 0; o < KG - 1; ++o) {
+#pragma unroll
+            for (int i = 0; i < FN * FM; ++i) acc[i / FM][i % FM] = acc[i / FM][i % FM] + *reinterpret_cast<const f32x4*>(sums + (o * GW + gwave) * SUMS + i * 1024 + lane * 16);
+        }
+    }
+    constexpr int ROW = TN / WN * static_cast<int>(elem_size<OUT>), CHUNKS = ROW / 16, PER = 16 / static_cast<int>(elem_size<OUT>);
+    constexpr bool WHOLE = KG == 1 && (CHUNKS == 8 || CHUNKS == 16) && TM / WM * ROW * WAVES <= 2 * STAGE;
+    if (!WHOLE || g.beta != 0.0f) {
+#pragma unroll
+        for (int i = 0; i < FN; ++i) {
+#pragma unroll
+            for (int j = 0; j < FM; ++j) store_four<OUT>(g, m0 + wm + 16 * j + lane % 16, n0 + wn + 16 * i + (lane / 16) * 4, acc[i][j]);
+        }
+        return;
+    }
+    if constexpr (WHOLE) {
+    // A wave's outputs pass through its own part of the stages, so that rows leave as whole runs of 16 bytes a lane:
+    // [row][16-byte chunk], chunk c of row r at place c ^ (r % CHUNKS).
+    __syncthreads();  // every wave is done with the stages
+    uint8_t* mine = &stages[0][0] + wave * (TM / WM * ROW);
+#pragma unroll
+    for (int i = 0; i < FN; ++i) {
+#pragma unroll
+        for (int j = 0; j < FM; ++j) {
+            const uint32_t r = 16 * j + lane % 16, byte = (16 * i + (lane / 16) * 4) * elem_size<OUT>;
+            uint8_t* to = mine + r * ROW + (((byte / 16) ^ (r % CHUNKS)) * 16 + byte % 16);
+            const f32x4 v = acc[i][j] * g.alpha;
+            if constexpr (OUT == LG_DTYPE_F32) {
+                *reinterpret_cast<f32x4*>(to) = v;
+            } else {
+                *reinterpret_cast<u32x2*>(to) = u32x2{pack2<OUT>(v[0], v[1]), pack2<OUT>(v[2], v[3])};
+            }
+        }
+    }
+    // The wave's own writes only: no other wave reads them.
+    __builtin_amdgcn_wave_barrier();
+    const uint32_t c = lane % CHUNKS, n = n0 + wn + c * PER;
+#pragma unroll
+    for (int q = 0; q < TM / WM * CHUNKS / 64; ++q) {
+        const uint32_t r = q * (64 / CHUNKS) + lane / CHUNKS, m = m0 + wm + r;
+        const u32x4 v = *reinterpret_cast<const u32x4*>(mine + r * ROW + (c ^ (r % CHUNKS)) * 16);
+        if (m >= g.m || n >= g.n) continue;
+        char* to = static_cast<char*>(g.c) + (m * g.c_pitch + n) * elem_size<OUT>;
+        if (n + PER <= g.n) {
+            *reinterpret_cast<u32x4_any*>(to) = v;
+        } else {
+            for (uint32_t e = 0; n + e < g.n; ++e) {
+                if constexpr (OUT == LG_DTYPE_F32) {
+                    reinterpret_cast<uint32_t*>(to)[e] = v[e];
+                } else {
+                    reinterpret_cast<uint16_t*>(to)[e] = static_cast<uint16_t>(v[e / 2] >> (16 * (e % 2)));
+                }
+            }
+        }
+    }
+    }
+}
+
+template <uint32_t OUT, bool DIRECT, bool FAST, bool E8M0, bool BROWS, int TM, int TN, int WM, int WN, int KG>
+void launch_tile(lg_ctx* ctx, hipStream_t s, const GemmBlocksArgs& g) {
+    const uint32_t tm = (g.m + TM - 1) / TM, tn = (g.n + TN - 1) / TN;
+    hipLaunchKernelGGL((gemm_blocks_tile<OUT, DIRECT, FAST, E8M0, BROWS, TM, TN, WM, WN, KG>), dim3(tm * tn), dim3(WM * WN * KG * 64), 0, s, g, tm, tn);
+    launched(ctx, FAST ? (TM == 256 ? (TN == 256 ? "gemm_blocks_fp8_256x256" : "gemm_blocks_fp8_256x128_any")
+                                    : (TM == 128 ? "gemm_blocks_fp8_128x128" : "gemm_blocks_fp8_64x64"))
+                       : (TM == 128 ? (DIRECT ? "gemm_blocks_bf16_128x128" : "gemm_blocks_bf16_128x128_any")
+                                    : TM == 64 ? (DIRECT ? "gemm_blocks_bf16_64x64" : "gemm_blocks_bf16_64x64_any")
+                                               : (DIRECT ? "gemm_blocks_bf16_32x64" : "gemm_blocks_bf16_32x64_any")));
+}
+
+// Few rows of A, at any address: a workgroup takes 16 FN rows of B and 16 FM of A, its W waves equal runs of
+// blocks, whose sums meet in LDS in the waves' order. Each byte of B goes from memory into the registers of the one
+// wave that multiplies it, 32 consecutive bytes a lane, the next block's while this one's is multiplied. Bound by
+// reading B: 1x65536x4096 39 us (6.9 TB/s), with FN = 1 and eight waves 45 us.
+template <uint32_t OUT, bool E8M0, bool BROWS, int FM, int FN, int W>
+__global__ __launch_bounds__(W * 64) void gemm_blocks_thin(GemmBlocksArgs g, uint32_t tiles_n) {
+    __shared__ f32x4 sums[W][FM * FN][64];
+    const uint32_t tid = threadIdx.x, lane = tid % 64, wave = __builtin_amdgcn_readfirstlane(tid / 64);
+    const uint32_t n0 = (blockIdx.x % tiles_n) * 16 * FN, m0 = (blockIdx.x / tiles_n) * 16 * FM;
+    const uint32_t blocks = (g.k + BLOCK_K - 1) / BLOCK_K, per = (blocks + W - 1) / W;
+    const uint32_t lo = min(wave * per, blocks), hi = min(lo + per, blocks);
+    const uint32_t row = lane % 16, part = (lane / 16) * 32;
+    const uint8_t* pa[FM];
+    const uint8_t* pb[FN];
+    const char* psa[FM];
+    const char* psb[FN][BROWS && !E8M0 ? 4 : 1];
+    constexpr int SIZE = E8M0 ? 1 : 4;
+#pragma unroll
+    for (int j = 0; j < FM; ++j) {
+        const uint32_t m = min(m0 + 16 * j + row, g.m - 1);
+        pa[j] = g.a + m * g.a_pitch + part;
+        psa[j] = static_cast<const char*>(g.sa) + (g.a_block == 1 ? m : m / BLOCK_K) * g.sa_pitch * SIZE;
+    }
+#pragma unroll
+    for (int i = 0; i < FN; ++i) {
+        const uint32_t n = min(n0 + 16 * i + row, g.n - 1);
+        pb[i] = g.b + n * g.b_pitch + part;
+        // e8m0 scales go with the lane's row of B, f32 ones with its four outputs' columns.
+        if constexpr (E8M0) {
+            psb[i][0] = static_cast<const char*>(g.sb) + (g.b_block == 1 ? n : n / BLOCK_K) * g.sb_pitch;
+        } else if constexpr (BROWS) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) psb[i][e] = static_cast<const char*>(g.sb) + min(n0 + 16 * i + (lane / 16) * 4 + e, g.n - 1) * g.sb_pitch * 4;
+        } else {
+            psb[i][0] = static_cast<const char*>(g.sb) + ((n0 + 16 * i) / BLOCK_K) * g.sb_pitch * 4;
+        }
+    }
+    f32x4 acc[FN][FM];
+#pragma unroll
+    for (int i = 0; i < FN; ++i) {
+#pragma unroll
+        for (int j = 0; j < FM; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    struct Slice {
+        u32x4 a[FM][2], b[FN][2];
+        float sa[FM], sb[FN][BROWS && !E8M0 ? 4 : 1];
+    };
+    auto load = [&](uint32_t kb, Slice& s) {
+        const uint32_t k = kb * BLOCK_K;
+        if (k + BLOCK_K <= g.k) {
+#pragma unroll
+            for (int i = 0; i < FN; ++i) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) s.b[i][h] = *reinterpret_cast<const u32x4_any*>(pb[i] + k + 16 * h);
+            }
+#pragma unroll
+            for (int j = 0; j < FM; ++j) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) s.a[j][h] = *reinterpret_cast<const u32x4_any*>(pa[j] + k + 16 * h);
+            }
+        } else {
+            for (int h = 0; h < 2; ++h) {
+                for (int i = 0; i < FN; ++i) s.b[i][h] = load_sixteen(pb[i] - part, k + part + 16 * h, g.k);
+                for (int j = 0; j < FM; ++j) s.a[j][h] = load_sixteen(pa[j] - part, k + part + 16 * h, g.k);
+            }
+        }
+        auto scale = [&](const char* p) { return E8M0 ? e8m0_value(reinterpret_cast<const uint8_t*>(p)[kb]) : reinterpret_cast<const float*>(p)[kb]; };
+#pragma unroll
+        for (int j = 0; j < FM; ++j) s.sa[j] = scale(psa[j]);
+#pragma unroll
+        for (int i = 0; i < FN; ++i) {
+#pragma unroll
+            for (int e = 0; e < (BROWS && !E8M0 ? 4 : 1); ++e) s.sb[i][e] = scale(psb[i][e]);
+        }
+    };
+    auto multiply = [&](const Slice& s) {
+        Fragment fb[FN];
+#pragma unroll
+        for (int i = 0; i < FN; ++i) fb[i] = Fragment(s.b[i][0], s.b[i][1], E8M0 ? s.sb[i][0] : 1.0f);
+#pragma unroll
+        for (int j = 0; j < FM; ++j) {
+            const Fragment fa(s.a[j][0], s.a[j][1], E8M0 ? s.sa[j] : 1.0f);
+#pragma unroll
+            for (int i = 0; i < FN; ++i) {
+                if constexpr (E8M0) {
+                    acc[i][j] = block_product(fb[i], fa, acc[i][j]);
+                } else {
+                    const f32x4 p = block_product(fb[i], fa);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) acc[i][j][e] = __builtin_fmaf(s.sa[j] * s.sb[i][BROWS ? e : 0], p[e], acc[i][j][e]);
+                }
+            }
+        }
+    };
+    if (lo < hi) {
+        Slice s[2];
+        load(lo, s[0]);
+        for (uint32_t kb = lo; kb < hi; kb += 2) {
+            if (kb + 1 < hi) load(kb + 1, s[1]);
+            multiply(s[0]);
+            if (kb + 1 >= hi) break;
+            if (kb + 2 < hi) load(kb + 2, s[0]);
+            multiply(s[1]);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < FN; ++i) {
+#pragma unroll
+        for (int j = 0; j < FM; ++j) sums[wave][i * FM + j][lane] = acc[i][j];
+    }
+    __syncthreads();
+    for (int q = wave; q < FM * FN; q += W) {
+        f32x4 v = sums[0][q][lane];
+#pragma unroll
+        for (int w = 1; w < W; ++w) v = v + sums[w][q][lane];
+        store_four<OUT>(g, m0 + 16 * (q % FM) + lane % 16, n0 + 16 * (q / FM) + (lane / 16) * 4, v);
+    }
+}
+
+template <uint32_t OUT, bool E8M0, bool BROWS, int FM, int FN, int W>
+void launch_thin(lg_ctx* ctx, hipStream_t s, const GemmBlocksArgs& g) {
+    const uint32_t tm = (g.m + 16 * FM - 1) / (16 * FM), tn = (g.n + 16 * FN - 1) / (16 * FN);
+    hipLaunchKernelGGL((gemm_blocks_thin<OUT, E8M0, BROWS, FM, FN, W>), dim3(tm * tn), dim3(W * 64), 0, s, g, tn);
+    launched(ctx, FN == 1 ? "gemm_blocks_thin16" : "gemm_blocks_thin32");
+}
+
+bool copies_fit(const GemmBlocksArgs& g) {
+    const uint64_t all = reinterpret_cast<uintptr_t>(g.a) | reinterpret_cast<uintptr_t>(g.b) | static_cast<uint64_t>(g.a_pitch) |
+                         static_cast<uint64_t>(g.b_pitch) | g.k;
+    return all % 16 == 0;
+}
+
+// The tile whose rounds over the compute units cost least: a round's time by block of K, measured on shapes of one
+// round (fewer than 256 tiles) and of many, in hundredths of a microsecond; `pair`: two workgroups share a
+// compute unit from 257 tiles on.
+struct Shape {
+    uint32_t tm, tn;
+    uint32_t round, pair;  // pair 0: one workgroup a compute unit
+};
+inline uint64_t cost(const GemmBlocksArgs& g, const Shape& s) {
+    const uint64_t tiles = static_cast<uint64_t>((g.m + s.tm - 1) / s.tm) * ((g.n + s.tn - 1) / s.tn);
+    if (s.pair == 0 || tiles <= 256) return (tiles + 255) / 256 * s.round;
+    return (tiles + 511) / 512 * s.pair;
+}
+constexpr Shape FP8_256{256, 256, 220, 0}, FP8_128{128, 128, 95, 140}, FP8_64{64, 64, 32, 60};
+constexpr Shape BF16_128{128, 128, 130, 210}, BF16_64{64, 64, 46, 85}, BF16_32{32, 64, 29, 0};
+// Operands that go through registers, timed at odd pitches.
+constexpr Shape FP8_256_ANY{256, 128, 240, 0}, BF16_128_ANY{128, 128, 170, 0}, BF16_64_ANY{64, 64, 75, 0}, BF16_32_ANY{32, 64, 55, 0};
+
+template <uint32_t OUT, bool E8M0, bool BROWS>
+void launch_of(lg_ctx* ctx, hipStream_t s, const GemmBlocksArgs& g) {
+    // Sixteen rows of A are one fragment: nothing of B is read twice, and LDS would only add to its way. Pitches from 2^23
+    // on come here too, since a tile's offsets would pass 32 bits.
+    if (g.m <= 16 || g.a_pitch >= (1 << 23) || g.b_pitch >= (1 << 23)) {
+        // From 8192 columns on two fragments of B to a wave fill the chip too, and share A's conversion (16x8192x4096:
+        // 9.0 us against 11.3); below, more waves share K (1x4096x4096: 4.8 us against 7.2).
+        if (g.n >= 8192) {
+            launch_thin<OUT, E8M0, BROWS, 1, 2, 4>(ctx, s, g);
+        } else {
+            launch_thin<OUT, E8M0, BROWS, 1, 1, 8>(ctx, s, g);
+        }
+        return;
+    }
+    const bool direct = copies_fit(g);
+    const uint64_t c128 = cost(g, direct ? BF16_128 : BF16_128_ANY), c64 = cost(g, direct ? BF16_64 : BF16_64_ANY), c32 = cost(g, direct ? BF16_32 : BF16_32_ANY);
+    if constexpr (OUT != LG_DTYPE_F32) {
+        // The fp8 instruction's precision is enough for 16-bit outputs of long sums.
+        if (g.k >= 512) {
+            if (direct) {
+                const uint64_t f256 = cost(g, FP8_256), f128 = cost(g, FP8_128), f64 = cost(g, FP8_64);
+                if (f256 <= f128 && f256 <= f64) {
+                    launch_tile<OUT, true, true, E8M0, BROWS, 256, 256, 4, 2, 1>(ctx, s, g);
+                    return;
+                }
+                if (f128 <= f64) {
+                    launch_tile<OUT, true, true, E8M0, BROWS, 128, 128, 2, 2, 1>(ctx, s, g);
+                    return;
+                }
+                if (f64 <= c32) {
+                    launch_tile<OUT, true, true, E8M0, BROWS, 64, 64, 2, 2, 2>(ctx, s, g);
+                    return;
+                }
+            } else if (const uint64_t f = cost(g, FP8_256_ANY); f <= c128 && f <= c64 && f <= c32) {
+                launch_tile<OUT, false, true, E8M0, BROWS, 256, 128, 4, 2, 1>(ctx, s, g);
+                return;
+            }
+        }
+    }
+    if (c128 <= c64 && c128 <= c32) {
+        direct ? launch_tile<OUT, true, false, E8M0, BROWS, 128, 128, 2, 2, 1>(ctx, s, g) : launch_tile<OUT, false, false, E8M0, BROWS, 128, 128, 4, 2, 1>(ctx, s, g);
+    } else if (c64 <= c32) {
+        direct ? launch_tile<OUT, true, false, E8M0, BROWS, 64, 64, 2, 2, 2>(ctx, s, g) : launch_tile<OUT, false, false, E8M0, BROWS, 64, 64, 2, 2, 2>(ctx, s, g);
+    } else {
+        direct ? launch_tile<OUT, true, false, E8M0, BROWS, 32, 64, 1, 4, 4>(ctx, s, g) : launch_tile<OUT, false, false, E8M0, BROWS, 32, 64, 1, 4, 4>(ctx, s, g);
+    }
+}
+
+}  // namespace
+
+template <uint32_t OUT>
+void launch_gemm_blocks_into(lg_ctx* ctx, hipStream_t s, const GemmBlocksArgs& g) {
+    if (g.e8m0) {
+        launch_of<OUT, true, true>(ctx, s, g);
+    } else if (g.b_block == 1) {
+        launch_of<OUT, false, true>(ctx, s, g);
+    } else {
+        launch_of<OUT, false, false>(ctx, s, g);
+    }
+}
+
+}  // namespace lg

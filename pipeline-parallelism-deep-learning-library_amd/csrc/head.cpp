@@ -10,6 +10,7 @@
 //                     the entry point says so, the transpose_matrix view of such a matrix
 //   Shape             an operand that reaches past its storage
 //   Alias             an output whose bytes intersect another operand's
+#include <algorithm>
 #include <cmath>
 
 #include "head.h"
@@ -162,6 +163,31 @@ void check_temperature(float t) {
 }
 
 uint32_t u32(uint64_t v) { return static_cast<uint32_t>(v); }
+
+// In parts whose tiles a launch has numbers for, whole blocks of 128 rows each.
+void launch_gemm_blocks(lg_ctx* ctx, hipStream_t s, const GemmBlocksArgs& g) {
+    constexpr uint32_t PART = 1u << 22;
+    const uint64_t scale = g.e8m0 ? 1 : 4, out = g.out == LG_DTYPE_F32 ? 4 : 2;
+    for (uint32_t m = 0; m < g.m; m += PART) {
+        for (uint32_t n = 0; n < g.n; n += PART) {
+            GemmBlocksArgs p = g;
+            p.m = std::min(g.m - m, PART);
+            p.n = std::min(g.n - n, PART);
+            p.a += m * g.a_pitch;
+            p.b += n * g.b_pitch;
+            p.sa = static_cast<const char*>(g.sa) + m / g.a_block * g.sa_pitch * scale;
+            p.sb = static_cast<const char*>(g.sb) + n / g.b_block * g.sb_pitch * scale;
+            p.c = static_cast<char*>(g.c) + (m * g.c_pitch + n) * out;
+            if (g.out == LG_DTYPE_F32) {
+                launch_gemm_blocks_f32(ctx, s, p);
+            } else if (g.out == LG_DTYPE_F16) {
+                launch_gemm_blocks_f16(ctx, s, p);
+            } else {
+                launch_gemm_blocks_bf16(ctx, s, p);
+            }
+        }
+    }
+}
 
 }  // namespace
 }  // namespace lg

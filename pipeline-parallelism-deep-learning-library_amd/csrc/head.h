@@ -1,5 +1,5 @@
 // Internal interfaces of a language model head's operators: the host's checks and plans (head.cpp)
-// and the kernels (quantize_kernels.hip, gemm_blocks_kernels.hip, logits_kernels.hip).
+// and the kernels (quantize_kernels.hip, gemm_blocks_*_kernels.hip, logits_kernels.hip).
 //
 // Every matrix is given by the address of its first element and a row pitch in elements; extents
 // fit 31 bits, and the host has proved that every element lies inside its storage.
@@ -41,7 +41,10 @@ struct GemmBlocksArgs {
     float alpha, beta;
     bool e8m0;
 };
-void launch_gemm_blocks(lg_ctx* ctx, hipStream_t s, const GemmBlocksArgs& args);
+// One for each type of c, in a file of its own; extents of C below 2^22.
+void launch_gemm_blocks_f32(lg_ctx* ctx, hipStream_t s, const GemmBlocksArgs& args);
+void launch_gemm_blocks_f16(lg_ctx* ctx, hipStream_t s, const GemmBlocksArgs& args);
+void launch_gemm_blocks_bf16(lg_ctx* ctx, hipStream_t s, const GemmBlocksArgs& args);
 
 struct LogprobArgs {
     const void* x;

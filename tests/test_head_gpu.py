@@ -149,6 +149,29 @@ def test_gemm_blocks_carries_what_is_not_a_number(hb, m, scales):
     product(hb, rng(600), m, 256, 256, scales, 1, 1, F32, spoil=spoil)
 
 
+PLANS = [
+    # m, n, k, out, the kernel that the plan's cost picks
+    (3, 1000, 700, F32, "thin16"), (16, 8200, 256, BF16, "thin32"), (40, 1024, 1024, F32, "bf16_32x64"),
+    (33, 1000, 301, F32, "bf16_32x64_any"), (1024, 1024, 256, F32, "bf16_64x64"), (1030, 1001, 127, F32, "bf16_64x64_any"),
+    (2048, 2560, 272, F32, "bf16_128x128"), (2049, 2561, 201, F16, "bf16_128x128_any"), (1024, 2048, 528, BF16, "fp8_64x64"),
+    (2048, 2048, 560, F16, "fp8_128x128"), (4100, 4090, 528, BF16, "fp8_128x128"), (4090, 4082, 528, BF16, "fp8_256x256"), (2050, 4099, 515, BF16, "fp8_256x128_any"),
+]
+
+
+@pytest.mark.parametrize("scales,ba,bb", [(F32, 1, 128), (F32, 128, 1), (E8M0, 1, 1)])
+@pytest.mark.parametrize("m,n,k,out,kernel", PLANS)
+def test_gemm_blocks_on_every_kernel(hb, m, n, k, out, kernel, scales, ba, bb):
+    product(hb, rng(700 + m), m, n, k, scales, ba, bb, out)
+    assert hb.debug_launches()[-1] == "gemm_blocks_" + kernel
+
+
+@pytest.mark.parametrize("m,n,k,out,kernel", PLANS)
+def test_gemm_blocks_on_every_kernel_into_what_is_there(hb, m, n, k, out, kernel):
+    """beta, and rows of C at an odd pitch and offset."""
+    any_address = kernel.endswith("_any")
+    product(hb, rng(710 + m), m, n, k, F32, 1, 128, out, 0.5, -1.0, pad=(1, 2, 3) if any_address else (0, 16, 3))
+
+
 def test_gemm_blocks_without_a_sum(hb):
     """K = 0 and alpha = 0: c = beta * c; alpha = 0 reads neither operand (here full of NaN)."""
     g = rng(610)
