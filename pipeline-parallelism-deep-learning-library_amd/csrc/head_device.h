@@ -60,6 +60,17 @@ struct Run {
 #pragma unroll
         for (int i = 0; i < static_cast<int>(elem_size<DT> / 2); ++i) w[i] = *reinterpret_cast<const u32x4_any*>(p + 16 * i);
     }
+    // Elements are widened from here on again, and not held as f32 since an earlier use.
+    __device__ inline void keep() {
+#pragma unroll
+        for (int i = 0; i < static_cast<int>(elem_size<DT> / 2); ++i) __asm__ volatile("" : "+v"(w[i]));
+    }
+    // Eight times -inf.
+    __device__ inline void clear() {
+        const uint32_t none = DT == LG_DTYPE_F32 ? 0xff800000u : DT == LG_DTYPE_BF16 ? 0xff80ff80u : 0xfc00fc00u;
+#pragma unroll
+        for (int i = 0; i < static_cast<int>(elem_size<DT> / 2); ++i) w[i] = u32x4{none, none, none, none};
+    }
     __device__ inline float operator[](int e) const {
         if constexpr (DT == LG_DTYPE_F32) {
             return __uint_as_float(w[e / 4][e % 4]);
