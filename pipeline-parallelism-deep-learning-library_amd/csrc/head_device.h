@@ -117,6 +117,42 @@ __device__ inline void store_run(char* p, const float (&v)[8]) {
     }
 }
 
+// A lane's value moved within the wave by a data-parallel step; `otherwise` where the step has no source.
+template <int STEP, int ROWS>
+__device__ inline float moved(float v, float otherwise) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(otherwise), __float_as_int(v), STEP, ROWS, 0xf, false));
+}
+template <int STEP, int ROWS>
+__device__ inline double moved(double v, double otherwise) {
+    const uint64_t a = __builtin_bit_cast(uint64_t, v), b = __builtin_bit_cast(uint64_t, otherwise);
+    const int lo = __builtin_amdgcn_update_dpp(static_cast<int>(b), static_cast<int>(a), STEP, ROWS, 0xf, false);
+    const int hi = __builtin_amdgcn_update_dpp(static_cast<int>(b >> 32), static_cast<int>(a >> 32), STEP, ROWS, 0xf, false);
+    return __builtin_bit_cast(double, static_cast<uint64_t>(static_cast<uint32_t>(hi)) << 32 | static_cast<uint32_t>(lo));
+}
+// Shifts by 1, 2, 4 and 8 within rows of sixteen lanes, then the last lane of a row to the next and of the lower half to
+// the upper: lane 63 ends with all. Every lane returns it.
+__device__ inline float wave_max(float v) {
+    v = fmaxf(v, moved<0x111, 0xf>(v, v));
+    v = fmaxf(v, moved<0x112, 0xf>(v, v));
+    v = fmaxf(v, moved<0x114, 0xf>(v, v));
+    v = fmaxf(v, moved<0x118, 0xf>(v, v));
+    v = fmaxf(v, moved<0x142, 0xa>(v, v));
+    v = fmaxf(v, moved<0x143, 0xc>(v, v));
+    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
+}
+__device__ inline double wave_sum(double v) {
+    v += moved<0x111, 0xf>(v, 0.0);
+    v += moved<0x112, 0xf>(v, 0.0);
+    v += moved<0x114, 0xf>(v, 0.0);
+    v += moved<0x118, 0xf>(v, 0.0);
+    v += moved<0x142, 0xa>(v, 0.0);
+    v += moved<0x143, 0xc>(v, 0.0);
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(b), 63));
+    const uint32_t hi = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(b >> 32), 63));
+    return __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
+}
+
 inline void launched(Context* ctx, const char* name) {
     check_hip(hipGetLastError(), name);
     note_launch(ctx, name);

@@ -21,12 +21,7 @@ namespace {
 
 using namespace head_detail;
 
-constexpr int THREADS = 512;
-constexpr int WAVES = THREADS / 64;
-constexpr int UNROLL = 4;               // slots a thread loads before it uses the first
-constexpr uint32_t MAX_LIST = 512;      // slots whose elements are looked at for the alternatives
-constexpr uint32_t MAX_KEYS = 8 * MAX_LIST;
-constexpr uint32_t SLOT_BYTES = 32768;  // LDS of the slots' maxima: 2 or 4 bytes each
+constexpr int UNROLL = 4;  // slots a thread loads before it uses the first
 constexpr uint32_t TICKETS = SK_COUNTER_BYTES / sizeof(uint32_t);
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr double LN2 = 0.69314718055994530942;
@@ -133,40 +128,50 @@ __device__ inline uint64_t key_of(float v, uint32_t index) { return static_cast<
 __device__ inline float key_value(uint64_t k) { return unorder(static_cast<uint32_t>(k >> 32)); }
 __device__ inline uint32_t key_index(uint64_t k) { return 0xffffffffu - static_cast<uint32_t>(k); }
 
+// What a workgroup of T threads, T / 64 waves, keeps in LDS.
+template <int T>
 struct Shared {
-    alignas(16) uint64_t wide[SLOT_BYTES / 8];  // the slots' maxima, then the candidates' keys
+    static constexpr int WAVES = T / 64;
+    static constexpr uint32_t SLOT_BYTES = T == 64 ? 4096 : 16384;  // of the slots' maxima: 2 or 4 bytes each
+    static constexpr uint32_t KEYS = SLOT_BYTES / 8;                // which take the maxima's place
+    static constexpr uint32_t LIST = T == 64 ? 64 : 512;            // slots whose elements are looked at
+    alignas(16) uint64_t wide[KEYS];
     uint64_t best[TOP_MAX];
-    float tops[THREADS];
-    uint32_t list[MAX_LIST];
+    float tops[T];
+    uint32_t list[LIST];
     double s[WAVES], u[WAVES];
     float m[WAVES];
-    uint32_t count, limit;
-    Part row;
+    float bound;  // below the k-th largest
+    uint32_t listed, found, count;
     bool last;
 };
-static_assert(MAX_KEYS * sizeof(uint64_t) <= SLOT_BYTES, "the keys take the maxima's place");
 
-// The largest of `tops` that at least k of them reach, to sixteen bits of its order and from below;
-// -inf where fewer than k are above -inf. By one wave.
+// The largest number that at least k of the N values in `tops` reach, to sixteen bits of its order and from below;
+// -inf where fewer than k are above -inf. Two bits a step, by one wave.
+template <int N>
 __device__ inline float threshold(const float* tops, uint32_t k) {
     const uint32_t lane = threadIdx.x % 64;
-    uint32_t o[THREADS / 64];
+    uint32_t o[N / 64];
 #pragma unroll
-    for (int i = 0; i < THREADS / 64; ++i) o[i] = order(tops[i * 64 + lane]) >> 16;
+    for (int i = 0; i < N / 64; ++i) o[i] = order(tops[i * 64 + lane]) >> 16;
     uint32_t t = 0;
-    for (uint32_t bit = 0x8000u; bit != 0; bit >>= 1) {
-        const uint32_t at = t | bit;
-        uint32_t n = 0;
 #pragma unroll
-        for (int i = 0; i < THREADS / 64; ++i) n += __popcll(__ballot(o[i] >= at));
-        if (n >= k) t = at;
+    for (int shift = 14; shift >= 0; shift -= 2) {
+        uint32_t n[3] = {0, 0, 0};
+#pragma unroll
+        for (uint32_t c = 0; c < 3; ++c) {
+#pragma unroll
+            for (int i = 0; i < N / 64; ++i) n[c] += __popcll(__ballot(o[i] >= (t | (c + 1) << shift)));
+        }
+        t |= (n[2] >= k ? 3u : n[1] >= k ? 2u : n[0] >= k ? 1u : 0u) << shift;
     }
     const float v = unorder(t << 16);
     return t <= 0x007fu ? -INF : v;
 }
 
 // How many of the workgroup's threads' `mine` there are in all.
-__device__ inline uint32_t total(Shared& sh, uint32_t mine) {
+template <int T>
+__device__ inline uint32_t total(Shared<T>& sh, uint32_t mine) {
     __syncthreads();
     if (threadIdx.x == 0) sh.count = 0;
     __syncthreads();
@@ -175,130 +180,146 @@ __device__ inline uint32_t total(Shared& sh, uint32_t mine) {
     return sh.count;
 }
 
-// sh.best = the k largest of the n keys in sh.wide, in order, then zeros. Keys differ from one another.
-__device__ inline void rank_keys(Shared& sh, uint32_t n, uint32_t k) {
-    for (uint32_t i = threadIdx.x; i < k; i += THREADS) sh.best[i] = 0;
+// The k-th largest of n keys that differ from one another, or 0 where there are fewer, bit by bit.
+template <int T, typename F>
+__device__ inline uint64_t kth_key(Shared<T>& sh, uint32_t n, uint32_t k, F&& key) {
+    uint64_t bound = 0;
+    for (uint64_t bit = 1ull << 63; bit != 0; bit >>= 1) {
+        uint32_t c = 0;
+        for (uint32_t i = threadIdx.x; i < n; i += T) c += key(i) >= (bound | bit) ? 1 : 0;
+        if (total(sh, c) >= k) bound |= bit;
+    }
     __syncthreads();
-    for (uint32_t i = threadIdx.x; i < n; i += THREADS) {
+    return bound;
+}
+
+// sh.best, zeros so far, = the k largest of the n keys in sh.wide, in order: each key goes to the place that as
+// many others exceed it, counted by four lanes. Keys differ from one another.
+template <int T>
+__device__ inline void rank_keys(Shared<T>& sh, uint32_t n, uint32_t k) {
+    constexpr uint32_t LANES = 4;
+    const uint32_t part = threadIdx.x % LANES;
+    for (uint32_t i = threadIdx.x / LANES; i < n; i += T / LANES) {
         const uint64_t mine = sh.wide[i];
         uint32_t above = 0;
-        for (uint32_t j = 0; j < n; ++j) above += sh.wide[j] > mine ? 1 : 0;
-        if (above < k) sh.best[above] = mine;
+#pragma unroll 4
+        for (uint32_t j = part; j < n; j += LANES) above += sh.wide[j] > mine ? 1 : 0;
+#pragma unroll
+        for (uint32_t d = 1; d < LANES; d *= 2) above += __shfl_xor(above, d);
+        if (part == 0 && above < k) sh.best[above] = mine;
     }
     __syncthreads();
 }
 
 // sh.best = the k largest keys of slots [lo, hi), whose maxima are in sh.wide and whose threads' maxima
-// are `mine`. An alternative lies in a slot whose maximum is one of the k largest, so slots below the
-// k-th largest of the threads' maxima drop out. Should more than MAX_LIST slots remain (many equal
-// logits), the k-th largest slot itself is found, bit by bit, with the slots that equal it taken from the
-// lowest.
-template <uint32_t DT>
-__device__ void top_of_slots(Shared& sh, const Slots<DT>& row, uint32_t lo, uint32_t hi, float mine, uint32_t k) {
+// are `mine`. An alternative lies in a slot whose maximum is one of the k largest, so slots below sh.bound, at
+// most the k-th largest of the threads' maxima, drop out. Should too much remain (many equal logits, or a few threads
+// with all of the largest), the k largest slots themselves are found, the lower of equal ones first. sh.listed and
+// sh.found are zero, sh.best zeros.
+template <uint32_t DT, int T>
+__device__ void top_of_slots(Shared<T>& sh, const Slots<DT>& row, uint32_t lo, uint32_t hi, float mine, uint32_t k) {
     typedef SlotMax<DT> Max;
     const typename Max::T* maxima = reinterpret_cast<const typename Max::T*>(sh.wide);
     const uint32_t tid = threadIdx.x, n = hi - lo;
-    sh.tops[tid] = mine;
-    if (tid == 0) sh.count = 0;
-    __syncthreads();
-    if (tid < 64) {
-        const float t = threshold(sh.tops, k);
-        if (tid == 0) sh.tops[0] = t;
-    }
-    __syncthreads();
-    float t = sh.tops[0];
+    float t = sh.bound;
     if (mine >= t) {
-        for (uint32_t i = tid; i < n; i += THREADS) {
+#pragma unroll 4
+        for (uint32_t i = tid; i < n; i += T) {
             const float v = Max::unpack(maxima[i]);
             if (v >= t && v > -INF) {
-                const uint32_t at = atomicAdd(&sh.count, 1u);
-                if (at < MAX_LIST) sh.list[at] = i;
+                const uint32_t at = atomicAdd(&sh.listed, 1u);
+                if (at < Shared<T>::LIST) sh.list[at] = i;
             }
         }
     }
     __syncthreads();
-    uint32_t listed = sh.count;
-    if (listed > MAX_LIST) {
-        uint32_t o = 0;
-        for (uint32_t bit = 0x80000000u; bit != 0; bit >>= 1) {
-            uint32_t c = 0;
-            for (uint32_t i = tid; i < n; i += THREADS) c += order(Max::unpack(maxima[i])) >= (o | bit) ? 1 : 0;
-            if (total(sh, c) >= k) o |= bit;
-        }
-        uint32_t c = 0;
-        for (uint32_t i = tid; i < n; i += THREADS) c += order(Max::unpack(maxima[i])) > o ? 1 : 0;
-        const uint32_t equal = k - total(sh, c);  // wanted from the slots whose maximum is the k-th: at least one
-        uint32_t end = 0;                         // slots below `end` hold fewer of them than that
-        for (uint32_t bit = 0x80000000u; bit != 0; bit >>= 1) {
-            const uint32_t at = end | bit;
-            if (at > n) continue;
-            c = 0;
-            for (uint32_t i = tid; i < at; i += THREADS) c += order(Max::unpack(maxima[i])) == o ? 1 : 0;
-            if (total(sh, c) < equal) end = at;
-        }
-        t = unorder(o);
-        __syncthreads();
-        if (tid == 0) sh.count = 0;
-        __syncthreads();
-        for (uint32_t i = tid; i < n; i += THREADS) {
-            const float v = Max::unpack(maxima[i]);
-            if (order(v) > o || (order(v) == o && i <= end)) sh.list[atomicAdd(&sh.count, 1u)] = i;
-        }
-        __syncthreads();
-        listed = sh.count;  // k
-    }
-    __syncthreads();
-    if (tid == 0) sh.count = 0;
-    __syncthreads();
-    for (uint32_t i = tid; i < listed * 8; i += THREADS) {
+    uint32_t listed = sh.listed;
+    // Element i % 8 of the list's slot i / 8, -inf for one outside the row.
+    auto element = [&](uint32_t i, uint32_t* index) {
         const uint32_t j = lo + sh.list[i / 8];
-        if (!row.has(j, i % 8)) continue;
-        const float v = load_one<DT>(row.base + (static_cast<uint64_t>(j) * 8 + i % 8) * elem_size<DT>);
-        if (v >= t && v > -INF) sh.wide[atomicAdd(&sh.count, 1u)] = key_of(v, row.first(j) + i % 8);
+        *index = row.first(j) + i % 8;
+        return row.has(j, i % 8) ? load_one<DT>(row.base + (static_cast<uint64_t>(j) * 8 + i % 8) * elem_size<DT>) : -INF;
+    };
+    bool many = listed > Shared<T>::LIST;
+    if (!many && listed * 8 > Shared<T>::KEYS) {
+        uint32_t c = 0, index;
+        for (uint32_t i = tid; i < listed * 8; i += T) c += element(i, &index) >= t ? 1 : 0;
+        many = total(sh, c) > Shared<T>::KEYS;
+    }
+    if (many) {
+        auto slot = [&](uint32_t i) { return key_of(Max::unpack(maxima[i]), i); };
+        const uint64_t bound = kth_key(sh, n, k, slot);
+        t = key_value(bound);
+        if (tid == 0) sh.listed = 0;
+        __syncthreads();
+        for (uint32_t i = tid; i < n; i += T) {
+            if (slot(i) >= bound) sh.list[atomicAdd(&sh.listed, 1u)] = i;
+        }
+        __syncthreads();
+        listed = sh.listed;  // k
+    }
+    for (uint32_t i = tid; i < listed * 8; i += T) {
+        uint32_t index;
+        const float v = element(i, &index);
+        if (v >= t && v > -INF) sh.wide[atomicAdd(&sh.found, 1u)] = key_of(v, index);
     }
     __syncthreads();
-    rank_keys(sh, sh.count, k);
+    rank_keys(sh, sh.found, k);
 }
 
-// The joined sums of the workgroup's threads, each relative to its own m.
-__device__ inline Part join(Shared& sh, float m, double s, double u, float c) {
+// The joined sums of the workgroup's threads, each relative to its own m; and for `k` > 0 in sh.bound at most the
+// k-th largest of the threads' values `mine`, which the first wave finds while the others add.
+template <bool ENTROPY, int T>
+__device__ inline Part join(Shared<T>& sh, float m, double s, double u, float c, uint32_t k, float mine) {
     const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64;
-    float top = m;
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
-    __syncthreads();
+    float top = wave_max(m);
     if (lane == 0) sh.m[wave] = top;
+    // For few alternatives the maxima of four threads bound the k-th largest closely enough.
+    const bool fold = T > 64 && k <= 24;
+    if (k > 0) {
+        if (fold) {
+            mine = fmaxf(mine, __shfl_xor(mine, 1));
+            mine = fmaxf(mine, __shfl_xor(mine, 2));
+        }
+        if (!fold || threadIdx.x % 4 == 0) sh.tops[fold ? threadIdx.x / 4 : threadIdx.x] = mine;
+    }
     __syncthreads();
+    if (k > 0 && wave == 0) {
+        float t;
+        if constexpr (T == 64) {
+            t = threshold<64>(sh.tops, k);
+        } else {
+            t = fold ? threshold<T / 4>(sh.tops, k) : threshold<T>(sh.tops, k);
+        }
+        if (lane == 0) sh.bound = t;
+    }
 #pragma unroll
-    for (int w = 0; w < WAVES; ++w) top = fmaxf(top, sh.m[w]);
+    for (int w = 0; w < Shared<T>::WAVES; ++w) top = fmaxf(top, sh.m[w]);
     if (m != -INF) {  // else s and u are zero, or NaN
         const float shift = (m - top) * c;
         const double f = exp2_fast(shift);
-        u = f * (u + fmaxf(shift, 4 * FAR) * s);
+        if (ENTROPY) u = f * (u + fmaxf(shift, 4 * FAR) * s);
         s = f * s;
     }
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-        s += __shfl_xor(s, d);
-        u += __shfl_xor(u, d);
-    }
+    s = wave_sum(s);
+    if (ENTROPY) u = wave_sum(u);
     if (lane == 0) {
         sh.s[wave] = s;
-        sh.u[wave] = u;
+        if (ENTROPY) sh.u[wave] = u;
     }
     __syncthreads();
     Part p{top, 0.0f, 0.0, 0.0};
 #pragma unroll
-    for (int w = 0; w < WAVES; ++w) {
+    for (int w = 0; w < Shared<T>::WAVES; ++w) {
         p.s += sh.s[w];
-        p.u += sh.u[w];
+        if (ENTROPY) p.u += sh.u[w];
     }
     return p;
 }
 
 // Writes what is asked of a row with sums p and, for k > 0, its best keys in sh.best.
-template <uint32_t DT>
-__device__ inline void finish_logprobs(const PassArgs& a, const Shared& sh, const char* x, uint32_t row, Part p) {
+template <int T>
+__device__ inline void finish_logprobs(const PassArgs& a, const Shared<T>& sh, bool named, float logit, uint32_t row, Part p) {
     const LogprobArgs& o = a.lp;
     const uint32_t tid = threadIdx.x;
     const bool bad = p.s != p.s, empty = !bad && p.m == -INF;
@@ -306,12 +327,8 @@ __device__ inline void finish_logprobs(const PassArgs& a, const Shared& sh, cons
     const float nan = __builtin_nanf("");
     if (tid == 0) {
         if (o.tokens != nullptr) {
-            const int32_t t = o.tokens[row];
             float v = 0.0f;
-            if (t >= 0 && static_cast<uint32_t>(t) < a.cols) {
-                const float d = load_one<DT>(x + static_cast<uint64_t>(t) * elem_size<DT>) - (empty ? 0.0f : p.m);
-                v = bad ? nan : static_cast<float>(static_cast<double>(d) / o.temperature - log_s);
-            }
+            if (named) v = bad ? nan : static_cast<float>(static_cast<double>(logit - (empty ? 0.0f : p.m)) / o.temperature - log_s);
             o.logprobs[row] = v;
         }
         if (o.entropy != nullptr) o.entropy[row] = bad ? nan : empty ? 0.0f : static_cast<float>(log_s - LN2 * (p.u / p.s));
@@ -320,7 +337,7 @@ __device__ inline void finish_logprobs(const PassArgs& a, const Shared& sh, cons
             o.stats[row * o.stats_pitch + 1] = bad ? nan : empty ? -INF : static_cast<float>(log_s);
         }
     }
-    for (uint32_t i = tid; i < o.k; i += THREADS) {
+    for (uint32_t i = tid; i < o.k; i += T) {
         const uint64_t key = bad ? 0 : sh.best[i];
         o.top_ids[row * o.ids_pitch + i] = key == 0 ? -1 : static_cast<int32_t>(key_index(key));
         const float v = key == 0 ? -INF : static_cast<float>(static_cast<double>(key_value(key) - p.m) / o.temperature - log_s);
@@ -372,16 +389,13 @@ struct Entries {
         norm = 0.0;
         if (!o.normalize) return;
         float top = fmaxf(named[0] ? value[0] : -INF, named[1] ? value[1] : -INF);
-#pragma unroll
-        for (int d = 1; d < 64; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
+        top = wave_max(top);
         double sum = 0.0;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             if (named[i]) sum += exp(static_cast<double>(value[i]) - top);
         }
-#pragma unroll
-        for (int d = 1; d < 64; d *= 2) sum += __shfl_xor(sum, d);
-        norm = top + log(sum);
+        norm = top + log(wave_sum(sum));
     }
     // The mass sum p_i and, relative to the student's normalizer, the loss: sum p_i (log p_i - (x_i - m) / T).
     __device__ inline void sums(const DistillArgs& o, float m, double* mass, double* loss) const {
@@ -393,11 +407,8 @@ struct Entries {
             *mass += q;
             if (q != 0.0) *loss += q * (lp - static_cast<double>(logit[i] - m) / o.temperature);
         }
-#pragma unroll
-        for (int d = 1; d < 64; d *= 2) {
-            *mass += __shfl_xor(*mass, d);
-            *loss += __shfl_xor(*loss, d);
-        }
+        *mass = wave_sum(*mass);
+        *loss = wave_sum(*loss);
     }
 };
 
@@ -413,39 +424,142 @@ __device__ inline RowInfo finish_distill(const DistillArgs& o, const Entries& li
 
 // This wave's device-scope stores have reached memory. They go past the L2 (each XCD has its own) and are
 // read past it by device-scope loads, so a ticket drawn after this says that they are there; a release fence
-// would write back the whole L2, which costs every workgroup 0.1 us in turn (48 rows of 100003, 528
-// workgroups: 42 us of 53).
+// would write back the whole L2, which costs every workgroup 0.1 us in turn (the pass over 48 rows of 100003, 528
+// workgroups: 42 us with it, 12 without).
 __device__ inline void written() {
     __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");
 }
 
-// One workgroup's part of one row; the row's last workgroup finishes it.
-template <uint32_t DT, bool ENTROPY, bool TOP, bool DISTILL>
-__global__ __launch_bounds__(THREADS) void row_pass(PassArgs a) {
-    __shared__ Shared sh;
-    const uint32_t tid = threadIdx.x, at = blockIdx.x / a.segs, seg = blockIdx.x % a.segs, row = a.row0 + at;
-    const char* x = a.x + row * a.x_pitch * elem_size<DT>;
+// The joined parts of row `at`, by the workgroup that wrote the last of them; with TOP their best keys in sh.best.
+template <bool ENTROPY, bool TOP, int T>
+__device__ Part join_parts(const PassArgs& a, Shared<T>& sh, uint32_t at) {
+    const uint32_t tid = threadIdx.x, k = TOP ? a.lp.k : 0, all = a.segs * k;
+    if (tid == 0) __hip_atomic_store(a.tickets + at, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    auto key = [&](uint32_t i) {
+        return __hip_atomic_load(a.part_keys + static_cast<uint64_t>(at) * all + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    };
+    // The threads' largest keys bound the k-th of all from below, closely where a thread's keys are of differing
+    // ranks in the parts' sorted lists. Up to HELD keys a thread stay in registers.
+    auto turn = [&](uint32_t i) { return i * T + (tid + 83 * i) % T; };
+    constexpr int HELD = 8;
+    uint64_t held[HELD];
+    float mine = -INF;
+    if constexpr (TOP) {
+#pragma unroll
+        for (int i = 0; i < HELD; ++i) held[i] = turn(i) < all ? key(turn(i)) : 0;
+#pragma unroll
+        for (int i = 0; i < HELD; ++i) mine = held[i] != 0 ? fmaxf(mine, key_value(held[i])) : mine;
+        for (uint32_t i = HELD; i * T < all; ++i) {
+            const uint64_t v = turn(i) < all ? key(turn(i)) : 0;
+            if (v != 0) mine = fmaxf(mine, key_value(v));
+        }
+        for (uint32_t i = tid; i < TOP_MAX; i += T) sh.best[i] = 0;
+        if (tid == 0) sh.found = 0;
+    }
+    // Each thread joins the parts of its turn, in order.
+    float m = -INF;
+    double s = 0.0, u = 0.0;
+    for (uint32_t i = tid; i < a.segs; i += T) {
+        const Part* q = a.parts + static_cast<uint64_t>(at) * a.segs + i;
+        const float qm = __hip_atomic_load(&q->m, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        const double qs = __hip_atomic_load(&q->s, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        const double qu = ENTROPY ? __hip_atomic_load(&q->u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0.0;
+        const float ref = fmaxf(m, qm);
+        const float f = ref == -INF ? 0.0f : fmaxf((m - ref) * a.c, 4 * FAR), g = ref == -INF ? 0.0f : fmaxf((qm - ref) * a.c, 4 * FAR);
+        u = exp2_fast(f) * (u + f * s) + exp2_fast(g) * (qu + g * qs);
+        s = exp2_fast(f) * s + exp2_fast(g) * qs;
+        m = ref;
+    }
+    const Part p = join<ENTROPY>(sh, m, s, u, a.c, k, mine);
+    if constexpr (TOP) {
+        const float t = sh.bound;
+        auto push = [&](uint64_t v) {
+            const uint32_t to = atomicAdd(&sh.found, 1u);
+            if (to < Shared<T>::KEYS) sh.wide[to] = v;
+        };
+#pragma unroll
+        for (int i = 0; i < HELD; ++i) {
+            if (held[i] != 0 && key_value(held[i]) >= t) push(held[i]);
+        }
+        for (uint32_t i = HELD * T + tid; i < all; i += T) {
+            const uint64_t v = key(i);
+            if (v != 0 && key_value(v) >= t) push(v);
+        }
+        __syncthreads();
+        if (sh.found > Shared<T>::KEYS) {  // many equal ones
+            const uint64_t bound = kth_key(sh, all, k, key);
+            if (tid == 0) sh.found = 0;
+            __syncthreads();
+            for (uint32_t i = tid; i < all; i += T) {
+                const uint64_t v = key(i);
+                if (v != 0 && v >= bound) push(v);
+            }
+            __syncthreads();
+        }
+        rank_keys(sh, sh.found, k);
+    }
+    return p;
+}
+
+// A workgroup's part of a row.
+template <uint32_t DT>
+struct Piece {
+    uint32_t at, seg, row;  // at: row - row0
+    const char* x;
+    Slots<DT> slots;
+    uint32_t lo, hi;  // slots of the part
+    bool live;        // a row without weight is not read
+    __device__ inline Piece(const PassArgs& a, uint32_t item)
+        : at(item / a.segs), seg(item % a.segs), row(a.row0 + at), x(a.x + row * a.x_pitch * elem_size<DT>), slots(x, a.cols) {
+        lo = min(seg * a.seg_slots, slots.count);
+        hi = min(lo + a.seg_slots, slots.count);
+        live = a.ds.weights == nullptr || a.ds.weights[row] != 0.0f;
+    }
+};
+
+// A pass over a part of a row; the row's last workgroup finishes it. Bound by reading the logits, and by the latency of
+// what follows a row's last slot, under which other rows' workgroups of the compute unit read: 4096 rows of 32768 bf16
+// 44 us without entropy and alternatives (6.0 TB/s), 51 us with entropy, 59 and 65 us with 20 and 64 alternatives (by
+// workgroups of eight waves 57, 67 and 73 us); one row of 131072 with 20 alternatives 10.4 us.
+template <uint32_t DT, bool ENTROPY, bool TOP, bool DISTILL, int T>
+__global__ __launch_bounds__(T) void row_pass(PassArgs a) {
+    __shared__ Shared<T> sh;
+    const uint32_t tid = threadIdx.x;
+    typename SlotMax<DT>::T* maxima = reinterpret_cast<typename SlotMax<DT>::T*>(sh.wide);
+    const Piece<DT> now(a, blockIdx.x);
     if constexpr (DISTILL) {
-        if (a.ds.weights != nullptr && a.ds.weights[row] == 0.0f) {  // a row without weight is not read
-            if (tid == 0 && seg == 0) {
-                a.ds.losses[row] = 0.0f;
-                if (a.info != nullptr) a.info[at] = RowInfo{0.0f, 0.0f, 0.0f, 0.0f};
+        if (!now.live) {
+            if (tid == 0 && now.seg == 0) {
+                a.ds.losses[now.row] = 0.0f;
+                if (a.info != nullptr) a.info[now.at] = RowInfo{0.0f, 0.0f, 0.0f, 0.0f};
             }
             return;
         }
     }
-    const Slots<DT> slots(x, a.cols);
-    const uint32_t lo = min(seg * a.seg_slots, slots.count), hi = min(lo + a.seg_slots, slots.count);
-    typename SlotMax<DT>::T* maxima = reinterpret_cast<typename SlotMax<DT>::T*>(sh.wide);
+    // What the row's end needs beside its sums is asked for here, so that its latency passes under the row's own.
+    Entries list;
+    float logit = 0.0f;
+    bool named = false;
+    if constexpr (DISTILL) {
+        if (tid < 64) list.load<DT>(a.ds, now.x, now.row);
+    } else if (a.lp.tokens != nullptr) {
+        const int32_t t = a.lp.tokens[now.row];
+        named = t >= 0 && static_cast<uint32_t>(t) < a.cols;
+        if (named) logit = load_one<DT>(now.x + static_cast<uint64_t>(t) * elem_size<DT>);
+    }
+    if constexpr (TOP) {
+        for (uint32_t i = tid; i < TOP_MAX; i += T) sh.best[i] = 0;
+        if (tid == 0) sh.listed = sh.found = 0;
+    }
     float m = -INF;
     double s = 0.0, u = 0.0;
-    for (uint32_t j0 = lo + tid; j0 < hi; j0 += THREADS * UNROLL) {
+    for (uint32_t j0 = now.lo + tid; j0 < now.hi; j0 += T * UNROLL) {
         Run<DT> r[UNROLL];
 #pragma unroll
         for (int i = 0; i < UNROLL; ++i) {
-            const uint32_t j = j0 + i * THREADS;
-            if (j < hi) {
-                slots.load(j, r[i]);
+            const uint32_t j = j0 + i * T;
+            if (j < now.hi) {
+                now.slots.load(j, r[i]);
             } else {
                 r[i].clear();
             }
@@ -456,12 +570,12 @@ __global__ __launch_bounds__(THREADS) void row_pass(PassArgs a) {
             float v = r[i][0];
 #pragma unroll
             for (int e = 1; e < 8; ++e) v = fmaxf(v, r[i][e]);
-            if (TOP && j0 + i * THREADS < hi) maxima[j0 + i * THREADS - lo] = SlotMax<DT>::pack(v);
+            if (TOP && j0 + i * T < now.hi) maxima[j0 + i * T - now.lo] = SlotMax<DT>::pack(v);
             top = fmaxf(top, v);
         }
         const float ref = top == -INF ? 0.0f : top, shift = fmaxf((m - ref) * a.c, 4 * FAR);
         const double f = exp2_fast(shift);
-        u = f * (u + shift * s);
+        if (ENTROPY) u = f * (u + shift * s);
         s = f * s;
 #pragma unroll
         for (int i = 0; i < UNROLL; ++i) {
@@ -477,81 +591,38 @@ __global__ __launch_bounds__(THREADS) void row_pass(PassArgs a) {
         }
         m = top;
     }
-    Part p = join(sh, m, s, u, a.c);
-    if constexpr (TOP) top_of_slots<DT>(sh, slots, lo, hi, m, a.lp.k);
+    Part p = join<ENTROPY>(sh, m, s, u, a.c, TOP ? a.lp.k : 0, m);
+    if constexpr (TOP) top_of_slots<DT>(sh, now.slots, now.lo, now.hi, m, a.lp.k);
     if (a.segs > 1) {
         // Thread 0 writes the part and draws the ticket; the keys are wave 0's.
         if (tid < 64) {
             if constexpr (TOP) {
-                uint64_t* keys = a.part_keys + (static_cast<uint64_t>(at) * a.segs + seg) * a.lp.k;
+                uint64_t* keys = a.part_keys + (static_cast<uint64_t>(now.at) * a.segs + now.seg) * a.lp.k;
                 for (uint32_t i = tid; i < a.lp.k; i += 64) __hip_atomic_store(keys + i, sh.best[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             }
             if (tid == 0) {
-                Part* to = a.parts + static_cast<uint64_t>(at) * a.segs + seg;
+                Part* to = a.parts + static_cast<uint64_t>(now.at) * a.segs + now.seg;
                 __hip_atomic_store(&to->m, p.m, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
                 __hip_atomic_store(&to->s, p.s, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                __hip_atomic_store(&to->u, p.u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                if (ENTROPY) __hip_atomic_store(&to->u, p.u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             }
             written();
-            if (tid == 0) sh.last = __hip_atomic_fetch_add(a.tickets + at, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == a.segs - 1;
+            if (tid == 0) sh.last = __hip_atomic_fetch_add(a.tickets + now.at, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == a.segs - 1;
         }
         __syncthreads();
         if (!sh.last) return;
-        if (tid == 0) __hip_atomic_store(a.tickets + at, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        // Each thread joins the parts of its turn, in order.
-        float jm = -INF;
-        double js = 0.0, ju = 0.0;
-        for (uint32_t i = tid; i < a.segs; i += THREADS) {
-            const Part* q = a.parts + static_cast<uint64_t>(at) * a.segs + i;
-            const float qm = __hip_atomic_load(&q->m, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            const double qs = __hip_atomic_load(&q->s, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            const double qu = __hip_atomic_load(&q->u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            const float ref = fmaxf(jm, qm);
-            const float f = ref == -INF ? 0.0f : fmaxf((jm - ref) * a.c, 4 * FAR), g = ref == -INF ? 0.0f : fmaxf((qm - ref) * a.c, 4 * FAR);
-            ju = exp2_fast(f) * (ju + f * js) + exp2_fast(g) * (qu + g * qs);
-            js = exp2_fast(f) * js + exp2_fast(g) * qs;
-            jm = ref;
-        }
-        p = join(sh, jm, js, ju, a.c);
-        if constexpr (TOP) {
-            const uint32_t k = a.lp.k, all = a.segs * k;
-            const uint64_t* keys = a.part_keys + static_cast<uint64_t>(at) * all;
-            // Each part's first few keys bound the k-th of all from below.
-            const uint32_t each = min(k, THREADS / a.segs), sg = tid / each;
-            float v = -INF;
-            if (each > 0 && sg < a.segs) {
-                const uint64_t key = __hip_atomic_load(keys + sg * k + tid % each, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                if (key != 0) v = key_value(key);
-            }
-            sh.tops[tid] = v;
-            if (tid == 0) sh.count = 0;
-            __syncthreads();
-            if (tid < 64) {
-                const float t = threshold(sh.tops, k);
-                if (tid == 0) sh.tops[0] = t;
-            }
-            __syncthreads();
-            const float t = sh.tops[0];
-            for (uint32_t i = tid; i < all; i += THREADS) {
-                const uint64_t key = __hip_atomic_load(keys + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                if (key != 0 && key_value(key) >= t) sh.wide[atomicAdd(&sh.count, 1u)] = key;
-            }
-            __syncthreads();
-            rank_keys(sh, sh.count, k);
-        }
+        p = join_parts<ENTROPY, TOP>(a, sh, now.at);
     }
     if constexpr (DISTILL) {
         if (tid < 64) {
-            Entries list;
-            list.load<DT>(a.ds, x, row);
             list.normalize(a.ds);
             double mass, loss;
             list.sums(a.ds, p.m, &mass, &loss);
-            const RowInfo info = finish_distill(a.ds, list, row, p, mass, loss);
-            if (a.info != nullptr && tid == 0) a.info[at] = info;
+            const RowInfo info = finish_distill(a.ds, list, now.row, p, mass, loss);
+            if (a.info != nullptr && tid == 0) a.info[now.at] = info;
         }
     } else {
-        finish_logprobs<DT>(a, sh, x, row, p);
+        finish_logprobs(a, sh, named, logit, now.row, p);
     }
 }
 
@@ -716,8 +787,7 @@ __global__ __launch_bounds__(T) void distill_rows(GradArgs a) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) top = fmaxf(top, r[i][e]);
         }
-#pragma unroll
-        for (int d = 1; d < 64; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
+        top = wave_max(top);
         if (lane == 0) tops[wave] = top;
         if (wave == 0) list.normalize(a.ds);
         __syncthreads();
@@ -733,8 +803,7 @@ __global__ __launch_bounds__(T) void distill_rows(GradArgs a) {
             for (int e = 0; e < 8; ++e) ps += exp2_fast((r[i][e] - ref) * a.c);
             s += ps;
         }
-#pragma unroll
-        for (int d = 1; d < 64; d *= 2) s += __shfl_xor(s, d);
+        s = wave_sum(s);
         if (lane == 0) sums[wave] = s;
         double mass = 0.0, loss = 0.0;
         if (wave == 0) list.sums(a.ds, top, &mass, &loss);
@@ -790,28 +859,34 @@ __global__ __launch_bounds__(T) void distill_rows(GradArgs a) {
 
 uint32_t ceil_div(uint64_t a, uint64_t b) { return static_cast<uint32_t>((a + b - 1) / b); }
 
-// Workgroups to a row: enough that rows of any number give every compute unit two, while each has at
-// least a slot for every thread; and where alternatives are wanted, no more slots than their maxima have
-// room for in LDS, and no more parts than the keys of.
+// Parts of a row, and slots to a part. Few rows are split until the chip has a workgroup for each compute unit, or two
+// while a part has over 64 KB, and each thread a slot; more only cost tickets (16 rows of 131072 in 256 parts 13.9 us, in
+// 512 15.9; 128 rows in 256 20.4, in 512 17.8). Where alternatives are wanted, no more slots than their maxima
+// have room for in LDS.
 struct Split {
     uint32_t segs, seg_slots;
 };
+constexpr int THREADS = 256;
 Split split_rows(uint32_t rows, uint32_t cols, uint32_t size, uint32_t k) {
-    const uint32_t slots = ceil_div(static_cast<uint64_t>(cols) + 7, 8) + 1, most = SLOT_BYTES / size;
-    uint32_t segs = rows >= 512 ? 1 : ceil_div(512, rows);
+    const uint32_t slots = ceil_div(static_cast<uint64_t>(cols) + 7, 8) + 1, most = Shared<THREADS>::SLOT_BYTES / size;
+    const uint32_t runs = static_cast<uint32_t>(static_cast<uint64_t>(cols) * size >> 16);
+    uint32_t segs = std::max(ceil_div(256, rows), std::min(ceil_div(512, rows), runs));
     segs = std::min(segs, ceil_div(slots, THREADS));
-    if (k > 0) {
-        segs = std::min(segs, MAX_KEYS / k);
-        segs = std::max(segs, ceil_div(slots, most));
-        if (static_cast<uint64_t>(segs) * k > MAX_KEYS) fail_invalid("token_logprobs: alternatives of so many logits do not fit");
-    }
+    if (k > 0) segs = std::max(std::min(segs, Shared<THREADS>::KEYS / k), ceil_div(slots, most));
     const uint32_t each = ceil_div(slots, segs);
     return {ceil_div(slots, each), each};
 }
 
 template <uint32_t DT, bool ENTROPY, bool TOP, bool DISTILL>
 void launch_pass(lg_ctx* ctx, hipStream_t s, const PassArgs& a, uint32_t rows) {
-    hipLaunchKernelGGL((row_pass<DT, ENTROPY, TOP, DISTILL>), dim3(rows * a.segs), dim3(THREADS), 0, s, a);
+    const uint32_t items = rows * a.segs;
+    // Many short rows: a wave each, whose 64 maxima bound few alternatives closely enough (4096 rows of 4096 with 5
+    // alternatives: 12.4 us, by workgroups of four waves 22 us).
+    if (a.segs == 1 && rows >= 1024 && a.seg_slots <= Shared<64>::SLOT_BYTES / elem_size<DT> && a.seg_slots <= 1025 && a.lp.k <= 24) {
+        hipLaunchKernelGGL((row_pass<DT, ENTROPY, TOP, DISTILL, 64>), dim3(items), dim3(64), 0, s, a);
+    } else {
+        hipLaunchKernelGGL((row_pass<DT, ENTROPY, TOP, DISTILL, THREADS>), dim3(items), dim3(THREADS), 0, s, a);
+    }
     launched(ctx, DISTILL ? "row_pass_distill" : TOP ? "row_pass_top" : "row_pass");
 }
 
@@ -819,7 +894,7 @@ void launch_pass(lg_ctx* ctx, hipStream_t s, const PassArgs& a, uint32_t rows) {
 template <typename F>
 void batches(uint32_t rows, uint64_t wgs_per_row, uint64_t most, F&& launch) {
     const uint64_t batch = std::min<uint64_t>(most, (1ull << 22) / wgs_per_row);
-    if (batch == 0) fail_invalid("rows of so many logits do not fit a launch");
+    if (batch == 0) fail_invalid("rows of so many logits do not fit a launch or its scratch");
     for (uint64_t r = 0; r < rows; r += batch) launch(static_cast<uint32_t>(r), static_cast<uint32_t>(std::min<uint64_t>(batch, rows - r)));
 }
 
