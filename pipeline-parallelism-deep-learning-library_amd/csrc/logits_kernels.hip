@@ -146,14 +146,22 @@ struct Shared {
     bool last;
 };
 
-// The largest number that at least k of the N values in `tops` reach, to sixteen bits of its order and from below;
-// -inf where fewer than k are above -inf. Two bits a step, by one wave.
-template <int N>
+// The largest number that at least k of `tops`' T values reach, to sixteen bits of its order and from below; -inf
+// where fewer than k are above -inf. FOLD: that many of the largest of each lane's values do. Two bits a step, by one wave.
+template <int T, bool FOLD>
 __device__ inline float threshold(const float* tops, uint32_t k) {
+    constexpr int N = FOLD ? 1 : T / 64;
     const uint32_t lane = threadIdx.x % 64;
-    uint32_t o[N / 64];
+    float v[T / 64];
 #pragma unroll
-    for (int i = 0; i < N / 64; ++i) o[i] = order(tops[i * 64 + lane]) >> 16;
+    for (int i = 0; i < T / 64; ++i) v[i] = tops[i * 64 + lane];
+    if (FOLD) {
+#pragma unroll
+        for (int i = 1; i < T / 64; ++i) v[0] = fmaxf(v[0], v[i]);
+    }
+    uint32_t o[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) o[i] = order(v[i]) >> 16;
     uint32_t t = 0;
 #pragma unroll
     for (int shift = 14; shift >= 0; shift -= 2) {
@@ -161,12 +169,11 @@ __device__ inline float threshold(const float* tops, uint32_t k) {
 #pragma unroll
         for (uint32_t c = 0; c < 3; ++c) {
 #pragma unroll
-            for (int i = 0; i < N / 64; ++i) n[c] += __popcll(__ballot(o[i] >= (t | (c + 1) << shift)));
+            for (int i = 0; i < N; ++i) n[c] += __popcll(__ballot(o[i] >= (t | (c + 1) << shift)));
         }
         t |= (n[2] >= k ? 3u : n[1] >= k ? 2u : n[0] >= k ? 1u : 0u) << shift;
     }
-    const float v = unorder(t << 16);
-    return t <= 0x007fu ? -INF : v;
+    return t <= 0x007fu ? -INF : unorder(t << 16);
 }
 
 // How many of the workgroup's threads' `mine` there are in all.
@@ -274,23 +281,11 @@ __device__ inline Part join(Shared<T>& sh, float m, double s, double u, float c,
     const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64;
     float top = wave_max(m);
     if (lane == 0) sh.m[wave] = top;
-    // For few alternatives the maxima of four threads bound the k-th largest closely enough.
-    const bool fold = T > 64 && k <= 24;
-    if (k > 0) {
-        if (fold) {
-            mine = fmaxf(mine, __shfl_xor(mine, 1));
-            mine = fmaxf(mine, __shfl_xor(mine, 2));
-        }
-        if (!fold || threadIdx.x % 4 == 0) sh.tops[fold ? threadIdx.x / 4 : threadIdx.x] = mine;
-    }
+    if (k > 0) sh.tops[threadIdx.x] = mine;
     __syncthreads();
     if (k > 0 && wave == 0) {
-        float t;
-        if constexpr (T == 64) {
-            t = threshold<64>(sh.tops, k);
-        } else {
-            t = fold ? threshold<T / 4>(sh.tops, k) : threshold<T>(sh.tops, k);
-        }
+        // For few alternatives the maxima of groups of threads bound the k-th largest closely enough.
+        const float t = k <= 24 ? threshold<T, true>(sh.tops, k) : threshold<T, false>(sh.tops, k);
         if (lane == 0) sh.bound = t;
     }
 #pragma unroll
