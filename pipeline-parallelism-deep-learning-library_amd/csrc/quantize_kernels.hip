@@ -7,6 +7,8 @@
 // once; e8m0 scales: s = 2^e, the smallest power of two with A <= 448 s, whose inverse is exact, so that
 // every element of a 16-bit or f32 matrix is rounded once. q = x * inv rounded to e4m3, to nearest,
 // ties to even (v_cvt_pk_fp8_f32); |x| * inv rounds to 448 at the most, so nothing overflows.
+#include <algorithm>
+
 #include "head_device.h"
 
 namespace lg {
@@ -104,69 +106,49 @@ __global__ __launch_bounds__(THREADS) void quantize_rows(QuantizeArgs a, uint32_
 }
 
 // A 128x128 tile of q by 256 threads: thread t holds eight runs of eight elements along the axis that
-// is contiguous in x. T: that axis is q's rows.
+// is contiguous in x. T: that axis is q's rows, and the tile turns in LDS, [row][128] with 8-byte run l of row r at place
+// l ^ (r / 8), so that q's rows leave in whole runs of 128 bytes. Neighbouring tiles of a row of them go to one
+// XCD, whose L2 then joins the lines that two tiles share.
 constexpr int TILE = 128;
 
 template <uint32_t DT, bool E8M0, bool T, bool BLOCK>
-__global__ __launch_bounds__(THREADS) void quantize_tile(QuantizeArgs a) {
-    const uint32_t r0 = blockIdx.y * TILE, c0 = blockIdx.x * TILE, tid = threadIdx.x;
+__global__ __launch_bounds__(THREADS) void quantize_tile(QuantizeArgs a, uint32_t tiles_c) {
+    static_assert(T || BLOCK, "rows of their own scales are quantize_rows'");
+    constexpr uint32_t XCDS = 8;
+    const uint32_t per = gridDim.x / XCDS, left = gridDim.x % XCDS, xcd = blockIdx.x % XCDS;
+    const uint32_t tile = xcd * per + min(xcd, left) + blockIdx.x / XCDS, tr = tile / tiles_c, tc = tile % tiles_c;
+    const uint32_t r0 = tr * TILE, c0 = tc * TILE, tid = threadIdx.x;
     const uint32_t along = tid % 16, line = tid / 16;
+    // Run i, T: column c0 + 8 line + i, rows r0 + 8 along ...; else row r0 + line + 16 i, columns c0 + 8 along ...
     float v[8][8];
     uint32_t top = 0;
-    if constexpr (!T) {
-        // Run i: row r0 + line + 16 i, columns c0 + 8 along ...
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const uint32_t r = r0 + line + 16 * i;
-            if (r < a.rows) {
-                load_eight<DT>(static_cast<const char*>(a.x) + r * a.x_pitch * elem_size<DT>, c0 + 8 * along, a.cols, v[i]);
-            } else {
+    for (int i = 0; i < 8; ++i) {
+        const uint32_t l = T ? c0 + 8 * line + i : r0 + line + 16 * i;
+        if (l < (T ? a.cols : a.rows)) {
+            load_eight<DT>(static_cast<const char*>(a.x) + l * a.x_pitch * elem_size<DT>, (T ? r0 : c0) + 8 * along, T ? a.rows : a.cols, v[i]);
+        } else {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) v[i][e] = 0.0f;
-            }
-#pragma unroll
-            for (int e = 0; e < 8; ++e) top = max(top, magnitude(v[i][e]));
-        }
-    } else {
-        // Run i: column c0 + 8 line + i, rows r0 + 8 along ...
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const uint32_t c = c0 + 8 * line + i;
-            if (c < a.cols) {
-                load_eight<DT>(static_cast<const char*>(a.x) + c * a.x_pitch * elem_size<DT>, r0 + 8 * along, a.rows, v[i]);
-            } else {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) v[i][e] = 0.0f;
-            }
-#pragma unroll
-            for (int e = 0; e < 8; ++e) top = max(top, magnitude(v[i][e]));
+            for (int e = 0; e < 8; ++e) v[i][e] = 0.0f;
         }
     }
+    float inverse[BLOCK ? 1 : 8];
     if constexpr (BLOCK) {
         __shared__ uint32_t tops[THREADS / 64];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) top = max(top, magnitude(v[i][e]));
+        }
 #pragma unroll
         for (int d = 1; d < 64; d *= 2) top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), d)));
         if (tid % 64 == 0) tops[tid / 64] = top;
         __syncthreads();
         top = max(max(tops[0], tops[1]), max(tops[2], tops[3]));
         const Scale<E8M0> s(top);
-        if (tid == 0) s.store(a.s, blockIdx.y * a.s_pitch + blockIdx.x);
-        if constexpr (!T) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const uint32_t r = r0 + line + 16 * i;
-                if (r < a.rows) store_eight(a.q + r * a.q_pitch, c0 + 8 * along, a.cols, to_e4m3(v[i], s.inverse));
-            }
-        } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const uint32_t r = r0 + 8 * along + e;
-                const float w[8] = {v[0][e], v[1][e], v[2][e], v[3][e], v[4][e], v[5][e], v[6][e], v[7][e]};
-                if (r < a.rows) store_eight(a.q + r * a.q_pitch, c0 + 8 * line, a.cols, to_e4m3(w, s.inverse));
-            }
-        }
+        if (tid == 0) s.store(a.s, tr * a.s_pitch + tc);
+        inverse[0] = s.inverse;
     } else {
-        static_assert(T || BLOCK, "rows of their own scales are quantize_rows'");
         // A scale for each of the tile's rows: the sixteen lines' maxima of a row meet in LDS.
         __shared__ uint32_t tops[16][TILE];
 #pragma unroll
@@ -177,21 +159,46 @@ __global__ __launch_bounds__(THREADS) void quantize_tile(QuantizeArgs a) {
             tops[line][8 * along + e] = m;
         }
         __syncthreads();
-        __shared__ float inverse[TILE];
+        __shared__ float inverses[TILE];
         if (tid < TILE) {
             uint32_t m = 0;
 #pragma unroll
             for (int i = 0; i < 16; ++i) m = max(m, tops[i][tid]);
             const Scale<E8M0> s(m);
-            inverse[tid] = s.inverse;
-            if (r0 + tid < a.rows) s.store(a.s, (r0 + tid) * a.s_pitch + blockIdx.x);
+            inverses[tid] = s.inverse;
+            if (r0 + tid < a.rows) s.store(a.s, (r0 + tid) * a.s_pitch + tc);
         }
         __syncthreads();
 #pragma unroll
+        for (int e = 0; e < 8; ++e) inverse[e] = inverses[8 * along + e];
+    }
+    if constexpr (!T) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const uint32_t r = r0 + line + 16 * i;
+            if (r < a.rows) store_eight(a.q + r * a.q_pitch, c0 + 8 * along, a.cols, to_e4m3(v[i], inverse[0]));
+        }
+    } else {
+        __shared__ u32x2 turned[TILE][16];
+#pragma unroll
         for (int e = 0; e < 8; ++e) {
-            const uint32_t r = r0 + 8 * along + e;
             const float w[8] = {v[0][e], v[1][e], v[2][e], v[3][e], v[4][e], v[5][e], v[6][e], v[7][e]};
-            if (r < a.rows) store_eight(a.q + r * a.q_pitch, c0 + 8 * line, a.cols, to_e4m3(w, inverse[8 * along + e]));
+            turned[8 * along + e][line ^ along] = to_e4m3(w, inverse[BLOCK ? 0 : e]);
+        }
+        __syncthreads();
+        const uint32_t chunk = tid % 8, c = c0 + 16 * chunk;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t l = tid / 8 + 32 * i, r = r0 + l;
+            if (r >= a.rows) break;
+            const u32x2 lo = turned[l][(2 * chunk) ^ (l / 8)], hi = turned[l][(2 * chunk + 1) ^ (l / 8)];
+            uint8_t* row = a.q + r * a.q_pitch;
+            if (c + 16 <= a.cols) {
+                *reinterpret_cast<u32x4_any*>(row + c) = u32x4{lo[0], lo[1], hi[0], hi[1]};
+            } else {
+                store_eight(row, c, a.cols, lo);
+                store_eight(row, c + 8, a.cols, hi);
+            }
         }
     }
 }
@@ -215,25 +222,26 @@ void launch_of(Context* ctx, hipStream_t s, const QuantizeArgs& a) {
         }
         return;
     }
-    // So do bands of rows beyond the grid's second extent.
-    constexpr uint32_t BANDS = 32768;
-    for (uint32_t b = 0; b < bands; b += BANDS) {
+    // So do bands of 128 rows.
+    const uint32_t most = (1u << 23) / groups;
+    if (most == 0) fail_invalid("quantize_blocks: a row of so many columns does not fit a launch");
+    for (uint32_t b = 0; b < bands; b += most) {
         QuantizeArgs p = a;
-        const uint64_t row = static_cast<uint64_t>(b) * TILE;
-        p.rows = static_cast<uint32_t>(a.rows - row);
-        if (p.rows > BANDS * TILE) p.rows = BANDS * TILE;
+        const int64_t row = static_cast<int64_t>(b) * TILE;
+        const uint32_t n = std::min(bands - b, most);
+        p.rows = static_cast<uint32_t>(std::min<int64_t>(a.rows - row, static_cast<int64_t>(n) * TILE));
         p.x = static_cast<const char*>(a.x) + row * (a.transposed ? 1 : a.x_pitch) * elem_size<DT>;
         p.q = a.q + row * a.q_pitch;
         p.s = static_cast<char*>(a.s) + (a.block == 1 ? row : b) * a.s_pitch * (E8M0 ? 1 : 4);
-        const dim3 grid(groups, (p.rows + TILE - 1) / TILE);
+        const dim3 grid(n * groups), threads(THREADS);
         if (a.block == 1) {
-            hipLaunchKernelGGL((quantize_tile<DT, E8M0, true, false>), grid, dim3(THREADS), 0, s, p);
+            hipLaunchKernelGGL((quantize_tile<DT, E8M0, true, false>), grid, threads, 0, s, p, groups);
             launched(ctx, "quantize_rows_t");
         } else if (a.transposed) {
-            hipLaunchKernelGGL((quantize_tile<DT, E8M0, true, true>), grid, dim3(THREADS), 0, s, p);
+            hipLaunchKernelGGL((quantize_tile<DT, E8M0, true, true>), grid, threads, 0, s, p, groups);
             launched(ctx, "quantize_tiles_t");
         } else {
-            hipLaunchKernelGGL((quantize_tile<DT, E8M0, false, true>), grid, dim3(THREADS), 0, s, p);
+            hipLaunchKernelGGL((quantize_tile<DT, E8M0, false, true>), grid, threads, 0, s, p, groups);
             launched(ctx, "quantize_tiles");
         }
     }
