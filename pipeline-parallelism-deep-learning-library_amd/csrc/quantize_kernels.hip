@@ -78,6 +78,24 @@ __device__ inline void load_eight(const char* p, uint32_t c, uint32_t cols, floa
     }
 }
 
+// The same of two runs of four, 64 columns apart.
+template <uint32_t DT>
+__device__ inline void load_halves(const char* p, uint32_t c, uint32_t cols, float (&v)[8]) {
+    static_assert(DT == LG_DTYPE_F32, "a lane's 16 bytes are four elements");
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const uint32_t at = c + 64 * h;
+        if (at + 4 <= cols) {
+            const u32x4 w = *reinterpret_cast<const u32x4_any*>(p + static_cast<uint64_t>(at) * 4);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[4 * h + e] = __uint_as_float(w[e]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[4 * h + e] = at + e < cols ? load_one<DT>(p + static_cast<uint64_t>(at + e) * 4) : 0.0f;
+        }
+    }
+}
+
 __device__ inline void store_eight(uint8_t* row, uint32_t c, uint32_t cols, u32x2 o) {
     if (c + 8 <= cols) {
         *reinterpret_cast<u32x2_any*>(row + c) = o;
@@ -106,7 +124,7 @@ __global__ __launch_bounds__(THREADS) void quantize_rows(QuantizeArgs a, uint32_
 }
 
 // A 128x128 tile of q by 256 threads: thread t holds eight runs of eight elements along the axis that
-// is contiguous in x. T: that axis is q's rows, and the tile turns in LDS, [row][128] with 8-byte run l of row r at place
+// is contiguous in x (of f32 two runs of four for T, so that a load of sixteen lanes is 256 bytes in a row). T: that axis is q's rows, and the tile turns in LDS, [row][128] with 8-byte run l of row r at place
 // l ^ (r / 8), so that q's rows leave in whole runs of 128 bytes. Neighbouring tiles of a row of them go to one
 // XCD, whose L2 then joins the lines that two tiles share.
 constexpr int TILE = 128;
@@ -119,6 +137,8 @@ __global__ __launch_bounds__(THREADS) void quantize_tile(QuantizeArgs a, uint32_
     const uint32_t tile = xcd * per + min(xcd, left) + blockIdx.x / XCDS, tr = tile / tiles_c, tc = tile % tiles_c;
     const uint32_t r0 = tr * TILE, c0 = tc * TILE, tid = threadIdx.x;
     const uint32_t along = tid % 16, line = tid / 16;
+    constexpr bool HALVES = T && DT == LG_DTYPE_F32;
+    auto row_of = [&](int e) { return HALVES ? 4 * along + e % 4 + 64 * (e / 4) : 8 * along + e; };  // T: element e's, in the tile
     // Run i, T: column c0 + 8 line + i, rows r0 + 8 along ...; else row r0 + line + 16 i, columns c0 + 8 along ...
     float v[8][8];
     uint32_t top = 0;
@@ -126,7 +146,12 @@ __global__ __launch_bounds__(THREADS) void quantize_tile(QuantizeArgs a, uint32_
     for (int i = 0; i < 8; ++i) {
         const uint32_t l = T ? c0 + 8 * line + i : r0 + line + 16 * i;
         if (l < (T ? a.cols : a.rows)) {
-            load_eight<DT>(static_cast<const char*>(a.x) + l * a.x_pitch * elem_size<DT>, (T ? r0 : c0) + 8 * along, T ? a.rows : a.cols, v[i]);
+            const char* p = static_cast<const char*>(a.x) + l * a.x_pitch * elem_size<DT>;
+            if constexpr (HALVES) {
+                load_halves<DT>(p, r0 + 4 * along, a.rows, v[i]);
+            } else {
+                load_eight<DT>(p, (T ? r0 : c0) + 8 * along, T ? a.rows : a.cols, v[i]);
+            }
         } else {
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[i][e] = 0.0f;
@@ -156,7 +181,7 @@ __global__ __launch_bounds__(THREADS) void quantize_tile(QuantizeArgs a, uint32_
             uint32_t m = 0;
 #pragma unroll
             for (int i = 0; i < 8; ++i) m = max(m, magnitude(v[i][e]));
-            tops[line][8 * along + e] = m;
+            tops[line][row_of(e)] = m;
         }
         __syncthreads();
         __shared__ float inverses[TILE];
@@ -170,7 +195,7 @@ __global__ __launch_bounds__(THREADS) void quantize_tile(QuantizeArgs a, uint32_
         }
         __syncthreads();
 #pragma unroll
-        for (int e = 0; e < 8; ++e) inverse[e] = inverses[8 * along + e];
+        for (int e = 0; e < 8; ++e) inverse[e] = inverses[row_of(e)];
     }
     if constexpr (!T) {
 #pragma unroll
@@ -183,7 +208,7 @@ __global__ __launch_bounds__(THREADS) void quantize_tile(QuantizeArgs a, uint32_
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             const float w[8] = {v[0][e], v[1][e], v[2][e], v[3][e], v[4][e], v[5][e], v[6][e], v[7][e]};
-            turned[8 * along + e][line ^ along] = to_e4m3(w, inverse[BLOCK ? 0 : e]);
+            turned[row_of(e)][line ^ (row_of(e) / 8)] = to_e4m3(w, inverse[BLOCK ? 0 : e]);
         }
         __syncthreads();
         const uint32_t chunk = tid % 8, c = c0 + 16 * chunk;
