@@ -88,23 +88,6 @@ __device__ inline void store_four(const GemmBlocksArgs& g, uint32_t m, uint32_t 
     }
 }
 
-// A TM x TN tile of C by KG groups of WM x WN waves. Slices of 128 columns lie in LDS as [row][128] with 16-byte
-// chunk c of row r at place c ^ (r & 7), so that eight neighbouring rows' reads of one chunk touch every bank once,
-// two stages of KG slices each. DIRECT (bases, pitches and K in whole 16 bytes): copied from memory straight into LDS
-// (global_load_lds_dwordx4) while the stage before is multiplied; else through registers, any addresses. Four copies
-// go out with each of the first rows of fragments, one row of B's fragments is read ahead, and a product joins its sum
-// two products later, so that neither LDS nor the multiply-adds keep the matrix cores waiting. A slice's scales
-// pass through registers into LDS beside it. Groups take slices in turn and add their sums in LDS at the end: more
-// waves for outputs of few tiles.
-// FAST multiplies on v_mfma_f32_16x16x128_f8f6f4, one instruction to a block of 16x16 outputs, at the precision
-// above; else in bf16.
-// Bound by the issue of LDS reads, multiply-adds and matrix instructions of two waves a SIMD; of few tiles by the
-// latency of a stage. Measured: 4096x65536x4096 into bf16, f32 scales on 256x256 tiles of eight waves, 1060 us (2080
-// TFLOP/s; a library product with one scale 840 us), e8m0 990 us; with rows of C stored by lanes as they hold them 1190 us,
-// with bands of eight tiles 1070 us. 8192x8192x4096 into f32 on 128x128 tiles of four waves, two workgroups a compute
-// unit: 513 us (1070 TFLOP/s), on 256x128 tiles 517 us; 8192x2048x4096 with e8m0 scales 125 us, multiplied in afterwards
-// 155 us. 512x2048x4096 into f32 on 64x64 tiles of two groups 18 us, on 128x128 tiles 40 us. 77x4099x2011 into f32
-// through registers on 32x64 tiles of four groups 12.2 us, on 64x64 tiles of two 16 us, of one 20 us.
 __device__ inline void copy_sixteen(const uint8_t* src, uint8_t* lds) { __builtin_amdgcn_global_load_lds(src, lds, 16, 0, 0); }
 
 typedef int i32x8 __attribute__((ext_vector_type(8)));
@@ -131,7 +114,7 @@ struct Operand<true> {
 // Workgroup `id` of `count` to a tile: neighbouring ids go to the eight XCDs in turn, so each XCD takes one
 // run of tiles, and runs walk bands of four tiles along M, whose operands its L2 then holds.
 __device__ inline void tile_of(uint32_t id, uint32_t tiles_m, uint32_t tiles_n, uint32_t* tm, uint32_t* tn) {
-        constexpr uint32_t XCDS = 8, BAND = 4;
+    constexpr uint32_t XCDS = 8, BAND = 4;
     const uint32_t count = tiles_m * tiles_n, per = count / XCDS, left = count % XCDS, xcd = id % XCDS;
     const uint32_t t = xcd * per + min(xcd, left) + id / XCDS;
     const uint32_t band = t / (BAND * tiles_n), first = band * BAND, high = min(BAND, tiles_m - first), in = t - first * tiles_n;
@@ -139,6 +122,23 @@ __device__ inline void tile_of(uint32_t id, uint32_t tiles_m, uint32_t tiles_n, 
     *tn = in / high;
 }
 
+// A TM x TN tile of C by KG groups of WM x WN waves. Slices of 128 columns lie in LDS as [row][128] with 16-byte
+// chunk c of row r at place c ^ (r & 7), so that eight neighbouring rows' reads of one chunk touch every bank once,
+// two stages of KG slices each. DIRECT (bases, pitches and K in whole 16 bytes): copied from memory straight into LDS
+// (global_load_lds_dwordx4) while the stage before is multiplied; else through registers, any addresses. Four copies
+// go out with each of the first rows of fragments, one row of B's fragments is read ahead, and a product joins its sum
+// two products later, so that neither LDS nor the multiply-adds keep the matrix cores waiting. A slice's scales
+// pass through registers into LDS beside it. Groups take slices in turn and add their sums in LDS at the end: more
+// waves for outputs of few tiles.
+// FAST multiplies on v_mfma_f32_16x16x128_f8f6f4, one instruction to a block of 16x16 outputs, at the precision
+// above; else in bf16.
+// Bound by the issue of LDS reads, multiply-adds and matrix instructions of two waves a SIMD; of few tiles by the
+// latency of a stage. Measured: 4096x65536x4096 into bf16, f32 scales on 256x256 tiles of eight waves, 1060 us (2080
+// TFLOP/s; a library product with one scale 840 us), e8m0 990 us; with rows of C stored by lanes as they hold them 1190 us,
+// with bands of eight tiles 1070 us. 8192x8192x4096 into f32 on 128x128 tiles of four waves, two workgroups a compute
+// unit: 513 us (1070 TFLOP/s), on 256x128 tiles 517 us; 8192x2048x4096 with e8m0 scales 125 us, multiplied in afterwards
+// 155 us. 512x2048x4096 into f32 on 64x64 tiles of two groups 18 us, on 128x128 tiles 40 us. 77x4099x2011 into f32
+// through registers on 32x64 tiles of four groups 12.2 us, on 64x64 tiles of two 16 us, of one 20 us.
 template <uint32_t OUT, bool DIRECT, bool FAST, bool E8M0, bool BROWS, int TM, int TN, int WM, int WN, int KG>
 __global__ __launch_bounds__(WM* WN * KG * 64) __attribute__((amdgpu_waves_per_eu(WM * WN * KG > 8 ? WM * WN * KG / 4 : 2))) void gemm_blocks_tile(GemmBlocksArgs g, uint32_t tiles_m, uint32_t tiles_n) {
     constexpr int WAVES = WM * WN * KG, T = WAVES * 64, FM = TM / WM / 16, FN = TN / WN / 16;

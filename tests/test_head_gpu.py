@@ -172,6 +172,26 @@ def test_gemm_blocks_on_every_kernel_into_what_is_there(hb, m, n, k, out, kernel
     product(hb, rng(710 + m), m, n, k, F32, 1, 128, out, 0.5, -1.0, pad=(1, 2, 3) if any_address else (0, 16, 3))
 
 
+@pytest.mark.parametrize("scales", [F32, E8M0])
+@pytest.mark.parametrize("m,n,k", [(200, 256, 640), (2050, 300, 515), (5, 200, 700)])
+def test_gemm_blocks_carries_what_is_not_a_number_into_16_bits(hb, m, n, k, scales):
+    def spoil(a, b):
+        a[1, 130] = np.inf
+        b[7, 5] = np.nan
+    product(hb, rng(630 + m), m, n, k, scales, 1, 1, BF16, spoil=spoil)
+
+
+@pytest.mark.parametrize("m,n,k", [(3, 200, 256), (200, 256, 256), (40, 70, 131)])
+def test_gemm_blocks_of_any_scale(hb, m, n, k):
+    """Rows whose sizes differ by 150 powers of two; products of two scales stay normal f32 numbers."""
+    g = rng(640 + m)
+    for scales in (F32, E8M0):
+        def spoil(a, b):
+            a *= np.exp2(g.integers(-60, 90, (m, 1))).astype(np.float32)
+            b *= np.float32(2.0 ** -30)
+        product(hb, g, m, n, k, scales, 1, 1, F32, spoil=spoil)
+
+
 def test_gemm_blocks_without_a_sum(hb):
     """K = 0 and alpha = 0: c = beta * c; alpha = 0 reads neither operand (here full of NaN)."""
     g = rng(610)
