@@ -48,15 +48,27 @@ __device__ inline float e8m0_value(uint32_t code) {
     return code == 255 ? __builtin_nanf("") : __uint_as_float(code == 0 ? 0x400000u : code << 23);
 }
 
-// Bytes k .. k + 15 of a row of length K at any address, zeros past its end.
+// Bytes k .. k + 15 of a row of length K at any address, zeros past its end: where they pass it, the row's last sixteen
+// shifted down. (Byte by byte under conditions, whose loads the compiler waits for one after another, 77x4099x2011 took 11.9 us
+// against 10.2, 1x4099x2011 8.3 against 6.1.)
 __device__ inline u32x4 load_sixteen(const uint8_t* row, uint32_t k, uint32_t K) {
     if (k + 16 <= K) return *reinterpret_cast<const u32x4_any*>(row + k);
     u32x4 v = {0, 0, 0, 0};
+    if (k >= K) return v;
+    if (K < 16) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-        if (k + i < K) v[i / 4] |= static_cast<uint32_t>(row[k + i]) << (8 * (i % 4));
+        for (uint32_t i = 0; i < 15; ++i) {
+            const uint32_t byte = row[min(k + i, K - 1)];
+            v[i / 4] |= (k + i < K ? byte : 0u) << (8 * (i % 4));
+        }
+        return v;
     }
-    return v;
+    v = *reinterpret_cast<const u32x4_any*>(row + K - 16);
+    const uint32_t shift = (k + 16 - K) * 8;  // 8 to 120
+    uint64_t lo = v[0] | static_cast<uint64_t>(v[1]) << 32, hi = v[2] | static_cast<uint64_t>(v[3]) << 32;
+    lo = shift < 64 ? lo >> shift | hi << (64 - shift) : hi >> (shift - 64);
+    hi = shift < 64 ? hi >> shift : 0;
+    return u32x4{static_cast<uint32_t>(lo), static_cast<uint32_t>(lo >> 32), static_cast<uint32_t>(hi), static_cast<uint32_t>(hi >> 32)};
 }
 
 // Outputs (m, n .. n + 3), those inside C, from the sums of a lane.
