@@ -13,6 +13,8 @@
 // conversion, or are the fp8 instruction's own operands.
 #pragma once
 
+#include <algorithm>
+
 #include "head_device.h"
 
 namespace lg {
@@ -141,7 +143,7 @@ __device__ inline void tile_of(uint32_t id, uint32_t tiles_m, uint32_t tiles_n, 
 // go out with each of the first rows of fragments, one row of B's fragments is read ahead, and a product joins its sum
 // two products later, so that neither LDS nor the multiply-adds keep the matrix cores waiting. A slice's scales
 // pass through registers into LDS beside it. Groups take slices in turn and add their sums in LDS at the end: more
-// waves for outputs of few tiles.
+// waves for outputs of few tiles. A group of one wave waits for no other until then.
 // FAST multiplies on v_mfma_f32_16x16x128_f8f6f4, one instruction to a block of 16x16 outputs, at the precision
 // above; else in bf16.
 // Bound by the issue of LDS reads, multiply-adds and matrix instructions of two waves a SIMD; of few tiles by the
@@ -149,8 +151,9 @@ __device__ inline void tile_of(uint32_t id, uint32_t tiles_m, uint32_t tiles_n, 
 // TFLOP/s; a library product with one scale 840 us), e8m0 990 us; with rows of C stored by lanes as they hold them 1190 us,
 // with bands of eight tiles 1070 us. 8192x8192x4096 into f32 on 128x128 tiles of four waves, two workgroups a compute
 // unit: 513 us (1070 TFLOP/s), on 256x128 tiles 517 us; 8192x2048x4096 with e8m0 scales 125 us, multiplied in afterwards
-// 155 us. 512x2048x4096 into f32 on 64x64 tiles of two groups 18 us, on 128x128 tiles 40 us. 77x4099x2011 into f32
-// through registers on 32x64 tiles of four groups 12.2 us, on 64x64 tiles of two 16 us, of one 20 us.
+// 155 us. 512x2048x4096 into f32 on 64x64 tiles of two groups 18 us, on 128x128 tiles 40 us; 256x256x4096 on 16x16 tiles of
+// sixteen groups 4.9 us, on 32x64 tiles of four 11.9 us. Through registers 77x4099x2011 on 32x64 tiles of four groups 10.2
+// us, on 32x32 tiles of eight, whose workgroups are more than the compute units, 14.5 us; 23x7261x1975 10.1 and 8.0 us.
 template <uint32_t OUT, bool DIRECT, bool FAST, bool E8M0, bool BROWS, int TM, int TN, int WM, int WN, int KG>
 __global__ __launch_bounds__(WM* WN * KG * 64) __attribute__((amdgpu_waves_per_eu(WM * WN * KG > 8 ? WM * WN * KG / 4 : 2))) void gemm_blocks_tile(GemmBlocksArgs g, uint32_t tiles_m, uint32_t tiles_n) {
     constexpr int WAVES = WM * WN * KG, T = WAVES * 64, FM = TM / WM / 16, FN = TN / WN / 16;
@@ -358,7 +361,11 @@ __global__ __launch_bounds__(WM* WN * KG * 64) __attribute__((amdgpu_waves_per_e
                 if (gtid + i * GW * 64 < TM + TN) sc[gtid + i * GW * 64] = next[i];
             }
         }
-        __syncthreads();
+        if constexpr (GW > 1) {
+            __syncthreads();
+        } else {
+            __asm__ volatile("" ::: "memory");  // a group of one wave reads its own slices only
+        }
         if (live) multiply(s % 2, (s + 1) * KG + kg < blocks, (s + 1) * KG + kg - 1);
     }
     if constexpr (KG > 1) {
@@ -433,39 +440,32 @@ __global__ __launch_bounds__(WM* WN * KG * 64) __attribute__((amdgpu_waves_per_e
 }
 
 template <uint32_t OUT, bool DIRECT, bool FAST, bool E8M0, bool BROWS, int TM, int TN, int WM, int WN, int KG>
-void launch_tile(lg_ctx* ctx, hipStream_t s, const GemmBlocksArgs& g) {
+void launch_tile(lg_ctx* ctx, hipStream_t s, const GemmBlocksArgs& g, const char* name) {
     const uint32_t tm = (g.m + TM - 1) / TM, tn = (g.n + TN - 1) / TN;
     hipLaunchKernelGGL((gemm_blocks_tile<OUT, DIRECT, FAST, E8M0, BROWS, TM, TN, WM, WN, KG>), dim3(tm * tn), dim3(WM * WN * KG * 64), 0, s, g, tm, tn);
-    launched(ctx, FAST ? (TM == 256 ? (TN == 256 ? "gemm_blocks_fp8_256x256" : "gemm_blocks_fp8_256x128_any")
-                                    : (TM == 128 ? "gemm_blocks_fp8_128x128" : "gemm_blocks_fp8_64x64"))
-                       : (TM == 128 ? (DIRECT ? "gemm_blocks_bf16_128x128" : "gemm_blocks_bf16_128x128_any")
-                                    : TM == 64 ? (DIRECT ? "gemm_blocks_bf16_64x64" : "gemm_blocks_bf16_64x64_any")
-                                               : (DIRECT ? "gemm_blocks_bf16_32x64" : "gemm_blocks_bf16_32x64_any")));
+    launched(ctx, name);
 }
 
-// Few rows of A, at any address: a workgroup takes 16 FN rows of B and 16 FM of A, its W waves equal runs of
+// Few rows of A, at any address: a workgroup takes 32 rows of B and 16 of A, its four waves equal runs of
 // blocks, whose sums meet in LDS in the waves' order. Each byte of B goes from memory into the registers of the one
-// wave that multiplies it, 32 consecutive bytes a lane, the next block's while this one's is multiplied. Bound by
-// reading B: 1x65536x4096 39 us (6.9 TB/s), with FN = 1 and eight waves 45 us.
-template <uint32_t OUT, bool E8M0, bool BROWS, int FM, int FN, int W>
+// wave that multiplies it, 32 consecutive bytes a lane, the next block's while this one's is multiplied. A lane reads a row
+// of its own, of which the caches serve a compute unit sixteen bytes a cycle: enough where every compute unit reads
+// (then bound by reading B: 1x65536x4096 46.6 us, 5.8 TB/s; 38.7 us of weights that the last call left in the caches),
+// too little where few do (1x4096x4096 7.3 us, on 16x16 tiles 4.7).
+template <uint32_t OUT, bool E8M0, bool BROWS, int FN, int W>
 __global__ __launch_bounds__(W * 64) void gemm_blocks_thin(GemmBlocksArgs g, uint32_t tiles_n) {
-    __shared__ f32x4 sums[W][FM * FN][64];
+    __shared__ f32x4 sums[W][FN][64];
     const uint32_t tid = threadIdx.x, lane = tid % 64, wave = __builtin_amdgcn_readfirstlane(tid / 64);
-    const uint32_t n0 = (blockIdx.x % tiles_n) * 16 * FN, m0 = (blockIdx.x / tiles_n) * 16 * FM;
+    const uint32_t n0 = (blockIdx.x % tiles_n) * 16 * FN, m0 = (blockIdx.x / tiles_n) * 16;
     const uint32_t blocks = (g.k + BLOCK_K - 1) / BLOCK_K, per = (blocks + W - 1) / W;
     const uint32_t lo = min(wave * per, blocks), hi = min(lo + per, blocks);
     const uint32_t row = lane % 16, part = (lane / 16) * 32;
-    const uint8_t* pa[FM];
     const uint8_t* pb[FN];
-    const char* psa[FM];
     const char* psb[FN][BROWS && !E8M0 ? 4 : 1];
     constexpr int SIZE = E8M0 ? 1 : 4;
-#pragma unroll
-    for (int j = 0; j < FM; ++j) {
-        const uint32_t m = min(m0 + 16 * j + row, g.m - 1);
-        pa[j] = g.a + m * g.a_pitch + part;
-        psa[j] = static_cast<const char*>(g.sa) + (g.a_block == 1 ? m : m / BLOCK_K) * g.sa_pitch * SIZE;
-    }
+    const uint32_t m = min(m0 + row, g.m - 1);
+    const uint8_t* pa = g.a + m * g.a_pitch + part;
+    const char* psa = static_cast<const char*>(g.sa) + (g.a_block == 1 ? m : m / BLOCK_K) * g.sa_pitch * SIZE;
 #pragma unroll
     for (int i = 0; i < FN; ++i) {
         const uint32_t n = min(n0 + 16 * i + row, g.n - 1);
@@ -480,15 +480,12 @@ __global__ __launch_bounds__(W * 64) void gemm_blocks_thin(GemmBlocksArgs g, uin
             psb[i][0] = static_cast<const char*>(g.sb) + ((n0 + 16 * i) / BLOCK_K) * g.sb_pitch * 4;
         }
     }
-    f32x4 acc[FN][FM];
+    f32x4 acc[FN];
 #pragma unroll
-    for (int i = 0; i < FN; ++i) {
-#pragma unroll
-        for (int j = 0; j < FM; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    }
+    for (int i = 0; i < FN; ++i) acc[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     struct Slice {
-        u32x4 a[FM][2], b[FN][2];
-        float sa[FM], sb[FN][BROWS && !E8M0 ? 4 : 1];
+        u32x4 a[2], b[FN][2];
+        float sa, sb[FN][BROWS && !E8M0 ? 4 : 1];
     };
     auto load = [&](uint32_t kb, Slice& s) {
         const uint32_t k = kb * BLOCK_K;
@@ -499,19 +496,15 @@ __global__ __launch_bounds__(W * 64) void gemm_blocks_thin(GemmBlocksArgs g, uin
                 for (int h = 0; h < 2; ++h) s.b[i][h] = *reinterpret_cast<const u32x4_any*>(pb[i] + k + 16 * h);
             }
 #pragma unroll
-            for (int j = 0; j < FM; ++j) {
-#pragma unroll
-                for (int h = 0; h < 2; ++h) s.a[j][h] = *reinterpret_cast<const u32x4_any*>(pa[j] + k + 16 * h);
-            }
+            for (int h = 0; h < 2; ++h) s.a[h] = *reinterpret_cast<const u32x4_any*>(pa + k + 16 * h);
         } else {
             for (int h = 0; h < 2; ++h) {
                 for (int i = 0; i < FN; ++i) s.b[i][h] = load_sixteen(pb[i] - part, k + part + 16 * h, g.k);
-                for (int j = 0; j < FM; ++j) s.a[j][h] = load_sixteen(pa[j] - part, k + part + 16 * h, g.k);
+                s.a[h] = load_sixteen(pa - part, k + part + 16 * h, g.k);
             }
         }
         auto scale = [&](const char* p) { return E8M0 ? e8m0_value(reinterpret_cast<const uint8_t*>(p)[kb]) : reinterpret_cast<const float*>(p)[kb]; };
-#pragma unroll
-        for (int j = 0; j < FM; ++j) s.sa[j] = scale(psa[j]);
+        s.sa = scale(psa);
 #pragma unroll
         for (int i = 0; i < FN; ++i) {
 #pragma unroll
@@ -519,21 +512,16 @@ __global__ __launch_bounds__(W * 64) void gemm_blocks_thin(GemmBlocksArgs g, uin
         }
     };
     auto multiply = [&](const Slice& s) {
-        Fragment fb[FN];
+        const Fragment fa(s.a[0], s.a[1], E8M0 ? s.sa : 1.0f);
 #pragma unroll
-        for (int i = 0; i < FN; ++i) fb[i] = Fragment(s.b[i][0], s.b[i][1], E8M0 ? s.sb[i][0] : 1.0f);
+        for (int i = 0; i < FN; ++i) {
+            const Fragment fb(s.b[i][0], s.b[i][1], E8M0 ? s.sb[i][0] : 1.0f);
+            if constexpr (E8M0) {
+                acc[i] = block_product(fb, fa, acc[i]);
+            } else {
+                const f32x4 p = block_product(fb, fa);
 #pragma unroll
-        for (int j = 0; j < FM; ++j) {
-            const Fragment fa(s.a[j][0], s.a[j][1], E8M0 ? s.sa[j] : 1.0f);
-#pragma unroll
-            for (int i = 0; i < FN; ++i) {
-                if constexpr (E8M0) {
-                    acc[i][j] = block_product(fb[i], fa, acc[i][j]);
-                } else {
-                    const f32x4 p = block_product(fb[i], fa);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) acc[i][j][e] = __builtin_fmaf(s.sa[j] * s.sb[i][BROWS ? e : 0], p[e], acc[i][j][e]);
-                }
+                for (int e = 0; e < 4; ++e) acc[i][e] = __builtin_fmaf(s.sa * s.sb[i][BROWS ? e : 0], p[e], acc[i][e]);
             }
         }
     };
@@ -549,24 +537,21 @@ __global__ __launch_bounds__(W * 64) void gemm_blocks_thin(GemmBlocksArgs g, uin
         }
     }
 #pragma unroll
-    for (int i = 0; i < FN; ++i) {
-#pragma unroll
-        for (int j = 0; j < FM; ++j) sums[wave][i * FM + j][lane] = acc[i][j];
-    }
+    for (int i = 0; i < FN; ++i) sums[wave][i][lane] = acc[i];
     __syncthreads();
-    for (int q = wave; q < FM * FN; q += W) {
+    for (int q = wave; q < FN; q += W) {
         f32x4 v = sums[0][q][lane];
 #pragma unroll
         for (int w = 1; w < W; ++w) v = v + sums[w][q][lane];
-        store_four<OUT>(g, m0 + 16 * (q % FM) + lane % 16, n0 + 16 * (q / FM) + (lane / 16) * 4, v);
+        store_four<OUT>(g, m0 + lane % 16, n0 + 16 * q + (lane / 16) * 4, v);
     }
 }
 
-template <uint32_t OUT, bool E8M0, bool BROWS, int FM, int FN, int W>
+template <uint32_t OUT, bool E8M0, bool BROWS, int FN, int W>
 void launch_thin(lg_ctx* ctx, hipStream_t s, const GemmBlocksArgs& g) {
-    const uint32_t tm = (g.m + 16 * FM - 1) / (16 * FM), tn = (g.n + 16 * FN - 1) / (16 * FN);
-    hipLaunchKernelGGL((gemm_blocks_thin<OUT, E8M0, BROWS, FM, FN, W>), dim3(tm * tn), dim3(W * 64), 0, s, g, tn);
-    launched(ctx, FN == 1 ? "gemm_blocks_thin16" : "gemm_blocks_thin32");
+    const uint32_t tm = (g.m + 15) / 16, tn = (g.n + 16 * FN - 1) / (16 * FN);
+    hipLaunchKernelGGL((gemm_blocks_thin<OUT, E8M0, BROWS, FN, W>), dim3(tm * tn), dim3(W * 64), 0, s, g, tn);
+    launched(ctx, "gemm_blocks_thin");
 }
 
 bool copies_fit(const GemmBlocksArgs& g) {
@@ -575,69 +560,96 @@ bool copies_fit(const GemmBlocksArgs& g) {
     return all % 16 == 0;
 }
 
-// The tile whose rounds over the compute units cost least: a round's time by block of K, measured on shapes of one
-// round (fewer than 256 tiles) and of many, in hundredths of a microsecond; `pair`: two workgroups share a
-// compute unit from 257 tiles on.
-struct Shape {
-    uint32_t tm, tn;
-    uint32_t round, pair;  // pair 0: one workgroup a compute unit
+// Which kernel is fastest is told by a model of its time: rounds of workgroups over the 256 compute units, each round a fixed
+// part and one for every turn of its groups along K. The figures, in hundredths of a microsecond, are a fit over 320
+// products with sizes spread evenly over the logarithms of 1 to 8192 rows, 128 to 16384 columns and K of 200 to 8192, each
+// timed on every kernel: the kernel with the least modelled time took 1.04 times the time of the fastest on
+// average. `share`: workgroups that share a compute unit, from 257 tiles on.
+struct Cost {
+    uint32_t m, n, groups, share;
+    struct {
+        uint32_t fixed, turn, shared_fixed, shared_turn;
+    } any, direct;  // through registers, timed at odd pitches; copied straight into LDS
 };
-inline uint64_t cost(const GemmBlocksArgs& g, const Shape& s) {
-    const uint64_t tiles = static_cast<uint64_t>((g.m + s.tm - 1) / s.tm) * ((g.n + s.tn - 1) / s.tn);
-    if (s.pair == 0 || tiles <= 256) return (tiles + 255) / 256 * s.round;
-    return (tiles + 511) / 512 * s.pair;
+enum Plan { THIN, BF16_128, BF16_64, BF16_32X64, BF16_32, BF16_16, FP8_256, FP8_128, FP8_64, FP8_32X64, FP8_32, PLANS };
+constexpr Cost COSTS[PLANS] = {
+    {16, 32, 4, 3, {76, 142, 0, 361}, {71, 55, 29, 135}},
+    {128, 128, 1, 2, {246, 133, 309, 314}, {177, 115, 314, 192}},
+    {64, 64, 2, 2, {134, 128, 270, 187}, {75, 88, 152, 145}},
+    {32, 64, 4, 1, {138, 157, 0, 0}, {107, 105, 0, 0}},
+    {32, 32, 8, 1, {134, 187, 0, 0}, {95, 113, 0, 0}},
+    {16, 16, 16, 1, {117, 160, 0, 0}, {78, 96, 0, 0}},
+    {256, 256, 1, 1, {0, 0, 0, 0}, {322, 150, 0, 0}},
+    {128, 128, 1, 2, {86, 122, 454, 187}, {155, 71, 227, 129}},
+    {64, 64, 2, 2, {92, 118, 120, 180}, {85, 58, 118, 113}},
+    {32, 64, 4, 1, {51, 164, 0, 0}, {97, 78, 0, 0}},
+    {32, 32, 8, 1, {136, 176, 0, 0}, {103, 87, 0, 0}},
+};
+inline Plan plan_of(const GemmBlocksArgs& g, bool direct) {
+    // Pitches from 2^23 on would pass 32 bits within a tile.
+    if (g.a_pitch >= (1 << 23) || g.b_pitch >= (1 << 23)) return THIN;
+    // The fp8 instruction's precision is enough for 16-bit outputs of long sums.
+    const bool fast = g.out != LG_DTYPE_F32 && g.k >= 512;
+    // Operands beyond the caches arrive at 6 TB/s for every kernel, soonest for the first.
+    const uint64_t reading = (static_cast<uint64_t>(g.m) + g.n) * g.k / 60000;
+    uint64_t best = ~0ull;
+    Plan plan = THIN;
+    for (int p = THIN; p < (fast ? PLANS : FP8_256); ++p) {
+        if (p == THIN ? g.m > 16 : p == FP8_256 && !direct) continue;
+        const Cost& c = COSTS[p];
+        const auto& t = direct ? c.direct : c.any;
+        const uint64_t tiles = static_cast<uint64_t>((g.m + c.m - 1) / c.m) * ((g.n + c.n - 1) / c.n);
+        const uint64_t turns = ((g.k + BLOCK_K - 1) / BLOCK_K + c.groups - 1) / c.groups;
+        uint64_t time = c.share == 1 || tiles <= 256 ? (tiles + 255) / 256 * (t.fixed + t.turn * turns)
+                                                     : (tiles + 256 * c.share - 1) / (256 * c.share) * (t.shared_fixed + t.shared_turn * turns);
+        time = std::max(time, reading);
+        if (time < best) {
+            best = time;
+            plan = static_cast<Plan>(p);
+        }
+    }
+    return plan;
 }
-constexpr Shape FP8_256{256, 256, 220, 0}, FP8_128{128, 128, 95, 140}, FP8_64{64, 64, 32, 60};
-constexpr Shape BF16_128{128, 128, 130, 210}, BF16_64{64, 64, 46, 85}, BF16_32{32, 64, 29, 0};
-// Operands that go through registers, timed at odd pitches.
-constexpr Shape FP8_256_ANY{256, 128, 240, 0}, BF16_128_ANY{128, 128, 170, 0}, BF16_64_ANY{64, 64, 75, 0}, BF16_32_ANY{32, 64, 55, 0};
+
+template <uint32_t OUT, bool DIRECT, bool E8M0, bool BROWS>
+void launch_of(lg_ctx* ctx, hipStream_t s, const GemmBlocksArgs& g) {
+    const Plan plan = plan_of(g, DIRECT);
+    if constexpr (OUT != LG_DTYPE_F32) {
+        switch (plan) {
+            case FP8_256:
+                if constexpr (DIRECT) launch_tile<OUT, true, true, E8M0, BROWS, 256, 256, 4, 2, 1>(ctx, s, g, "gemm_blocks_fp8_256x256");
+                return;
+            case FP8_128:
+                return launch_tile<OUT, DIRECT, true, E8M0, BROWS, 128, 128, DIRECT ? 2 : 4, 2, 1>(ctx, s, g, DIRECT ? "gemm_blocks_fp8_128x128" : "gemm_blocks_fp8_128x128_any");
+            case FP8_64:
+                return launch_tile<OUT, DIRECT, true, E8M0, BROWS, 64, 64, 2, 2, 2>(ctx, s, g, DIRECT ? "gemm_blocks_fp8_64x64" : "gemm_blocks_fp8_64x64_any");
+            case FP8_32X64:
+                return launch_tile<OUT, DIRECT, true, E8M0, BROWS, 32, 64, 1, 4, 4>(ctx, s, g, DIRECT ? "gemm_blocks_fp8_32x64" : "gemm_blocks_fp8_32x64_any");
+            case FP8_32:
+                return launch_tile<OUT, DIRECT, true, E8M0, BROWS, 32, 32, 1, 2, 8>(ctx, s, g, DIRECT ? "gemm_blocks_fp8_32x32" : "gemm_blocks_fp8_32x32_any");
+            default:
+                break;
+        }
+    }
+    switch (plan) {
+        case BF16_128:
+            return launch_tile<OUT, DIRECT, false, E8M0, BROWS, 128, 128, DIRECT ? 2 : 4, 2, 1>(ctx, s, g, DIRECT ? "gemm_blocks_bf16_128x128" : "gemm_blocks_bf16_128x128_any");
+        case BF16_64:
+            return launch_tile<OUT, DIRECT, false, E8M0, BROWS, 64, 64, 2, 2, 2>(ctx, s, g, DIRECT ? "gemm_blocks_bf16_64x64" : "gemm_blocks_bf16_64x64_any");
+        case BF16_32X64:
+            return launch_tile<OUT, DIRECT, false, E8M0, BROWS, 32, 64, 1, 4, 4>(ctx, s, g, DIRECT ? "gemm_blocks_bf16_32x64" : "gemm_blocks_bf16_32x64_any");
+        case BF16_32:
+            return launch_tile<OUT, DIRECT, false, E8M0, BROWS, 32, 32, 1, 2, 8>(ctx, s, g, DIRECT ? "gemm_blocks_bf16_32x32" : "gemm_blocks_bf16_32x32_any");
+        case BF16_16:
+            return launch_tile<OUT, DIRECT, false, E8M0, BROWS, 16, 16, 1, 1, 16>(ctx, s, g, DIRECT ? "gemm_blocks_bf16_16x16" : "gemm_blocks_bf16_16x16_any");
+        default:
+            return launch_thin<OUT, E8M0, BROWS, 2, 4>(ctx, s, g);
+    }
+}
 
 template <uint32_t OUT, bool E8M0, bool BROWS>
-void launch_of(lg_ctx* ctx, hipStream_t s, const GemmBlocksArgs& g) {
-    // Sixteen rows of A are one fragment: nothing of B is read twice, and LDS would only add to its way. Pitches from 2^23
-    // on come here too, since a tile's offsets would pass 32 bits.
-    if (g.m <= 16 || g.a_pitch >= (1 << 23) || g.b_pitch >= (1 << 23)) {
-        // From 8192 columns on two fragments of B to a wave fill the chip too, and share A's conversion (16x8192x4096:
-        // 9.0 us against 11.3); below, more waves share K (1x4096x4096: 4.8 us against 7.2).
-        if (g.n >= 8192) {
-            launch_thin<OUT, E8M0, BROWS, 1, 2, 4>(ctx, s, g);
-        } else {
-            launch_thin<OUT, E8M0, BROWS, 1, 1, 8>(ctx, s, g);
-        }
-        return;
-    }
-    const bool direct = copies_fit(g);
-    const uint64_t c128 = cost(g, direct ? BF16_128 : BF16_128_ANY), c64 = cost(g, direct ? BF16_64 : BF16_64_ANY), c32 = cost(g, direct ? BF16_32 : BF16_32_ANY);
-    if constexpr (OUT != LG_DTYPE_F32) {
-        // The fp8 instruction's precision is enough for 16-bit outputs of long sums.
-        if (g.k >= 512) {
-            if (direct) {
-                const uint64_t f256 = cost(g, FP8_256), f128 = cost(g, FP8_128), f64 = cost(g, FP8_64);
-                if (f256 <= f128 && f256 <= f64) {
-                    launch_tile<OUT, true, true, E8M0, BROWS, 256, 256, 4, 2, 1>(ctx, s, g);
-                    return;
-                }
-                if (f128 <= f64) {
-                    launch_tile<OUT, true, true, E8M0, BROWS, 128, 128, 2, 2, 1>(ctx, s, g);
-                    return;
-                }
-                if (f64 <= c32) {
-                    launch_tile<OUT, true, true, E8M0, BROWS, 64, 64, 2, 2, 2>(ctx, s, g);
-                    return;
-                }
-            } else if (const uint64_t f = cost(g, FP8_256_ANY); f <= c128 && f <= c64 && f <= c32) {
-                launch_tile<OUT, false, true, E8M0, BROWS, 256, 128, 4, 2, 1>(ctx, s, g);
-                return;
-            }
-        }
-    }
-    if (c128 <= c64 && c128 <= c32) {
-        direct ? launch_tile<OUT, true, false, E8M0, BROWS, 128, 128, 2, 2, 1>(ctx, s, g) : launch_tile<OUT, false, false, E8M0, BROWS, 128, 128, 4, 2, 1>(ctx, s, g);
-    } else if (c64 <= c32) {
-        direct ? launch_tile<OUT, true, false, E8M0, BROWS, 64, 64, 2, 2, 2>(ctx, s, g) : launch_tile<OUT, false, false, E8M0, BROWS, 64, 64, 2, 2, 2>(ctx, s, g);
-    } else {
-        direct ? launch_tile<OUT, true, false, E8M0, BROWS, 32, 64, 1, 4, 4>(ctx, s, g) : launch_tile<OUT, false, false, E8M0, BROWS, 32, 64, 1, 4, 4>(ctx, s, g);
-    }
+void launch_at(lg_ctx* ctx, hipStream_t s, const GemmBlocksArgs& g) {
+    copies_fit(g) ? launch_of<OUT, true, E8M0, BROWS>(ctx, s, g) : launch_of<OUT, false, E8M0, BROWS>(ctx, s, g);
 }
 
 }  // namespace
@@ -645,11 +657,11 @@ void launch_of(lg_ctx* ctx, hipStream_t s, const GemmBlocksArgs& g) {
 template <uint32_t OUT>
 void launch_gemm_blocks_into(lg_ctx* ctx, hipStream_t s, const GemmBlocksArgs& g) {
     if (g.e8m0) {
-        launch_of<OUT, true, true>(ctx, s, g);
+        launch_at<OUT, true, true>(ctx, s, g);
     } else if (g.b_block == 1) {
-        launch_of<OUT, false, true>(ctx, s, g);
+        launch_at<OUT, false, true>(ctx, s, g);
     } else {
-        launch_of<OUT, false, false>(ctx, s, g);
+        launch_at<OUT, false, false>(ctx, s, g);
     }
 }
 
