@@ -128,6 +128,8 @@ __device__ inline uint64_t key_of(float v, uint32_t index) { return static_cast<
 __device__ inline float key_value(uint64_t k) { return unorder(static_cast<uint32_t>(k >> 32)); }
 __device__ inline uint32_t key_index(uint64_t k) { return 0xffffffffu - static_cast<uint32_t>(k); }
 
+typedef uint64_t u64x2 __attribute__((ext_vector_type(2)));
+
 // What a workgroup of T threads, T / 64 waves, keeps in LDS.
 template <int T>
 struct Shared {
@@ -142,7 +144,7 @@ struct Shared {
     double s[WAVES], u[WAVES];
     float m[WAVES];
     float bound;  // below the k-th largest
-    uint32_t listed, found, count;
+    uint32_t listed, found, count, counts[24];
     bool last;
 };
 
@@ -200,17 +202,67 @@ __device__ inline uint64_t kth_key(Shared<T>& sh, uint32_t n, uint32_t k, F&& ke
     return bound;
 }
 
+// Keeps of the n keys in sh.wide those that can be among the k largest, told by the first sixteen bits, or where equal
+// ones are too many by all; returns how many.
+template <int T>
+__device__ uint32_t narrow(Shared<T>& sh, uint32_t n, uint32_t k) {
+    constexpr uint32_t HELD = Shared<T>::KEYS / T, STEPS = 8;
+    uint64_t held[HELD];
+#pragma unroll
+    for (uint32_t i = 0; i < HELD; ++i) held[i] = i * T + threadIdx.x < n ? sh.wide[i * T + threadIdx.x] : 0;
+    auto keep = [&](uint64_t bound) {
+        __syncthreads();
+        if (threadIdx.x == 0) sh.found = 0;
+        __syncthreads();
+#pragma unroll
+        for (uint32_t i = 0; i < HELD; ++i) {
+            if (held[i] != 0 && held[i] >= bound) sh.wide[atomicAdd(&sh.found, 1u)] = held[i];
+        }
+        __syncthreads();
+        return sh.found;
+    };
+    if (threadIdx.x < 3 * STEPS) sh.counts[threadIdx.x] = 0;
+    __syncthreads();
+    uint64_t t = 0;
+    for (uint32_t step = 0; step < STEPS; ++step) {
+        const uint32_t shift = 62 - 2 * step;
+#pragma unroll
+        for (uint64_t c = 0; c < 3; ++c) {
+            uint32_t above = 0;
+#pragma unroll
+            for (uint32_t i = 0; i < HELD; ++i) above += __popcll(__ballot(held[i] >= (t | (c + 1) << shift)));
+            if (threadIdx.x % 64 == 0) atomicAdd(&sh.counts[3 * step + c], above);
+        }
+        __syncthreads();
+        const uint32_t* count = sh.counts + 3 * step;
+        t |= (count[2] >= k ? 3ull : count[1] >= k ? 2ull : count[0] >= k ? 1ull : 0ull) << shift;
+    }
+    n = keep(t);
+    if (n <= 2 * T) return n;
+    const uint64_t bound = kth_key(sh, n, k, [&](uint32_t i) { return sh.wide[i]; });
+    return keep(bound);
+}
+
 // sh.best, zeros so far, = the k largest of the n keys in sh.wide, in order: each key goes to the place that as
-// many others exceed it, counted by four lanes. Keys differ from one another.
+// many others exceed it, counted by four lanes, sixteen pairs at a time. Keys differ from one another.
 template <int T>
 __device__ inline void rank_keys(Shared<T>& sh, uint32_t n, uint32_t k) {
-    constexpr uint32_t LANES = 4;
-    const uint32_t part = threadIdx.x % LANES;
+    constexpr uint32_t LANES = 4, PAIRS = 8;
+    if (n > 2 * T) n = narrow(sh, n, k);  // a row of 1000 with 128 alternatives, all of them keys, 13 us; by ranks alone 48
+    const uint32_t part = threadIdx.x % LANES, end = (n + 2 * LANES * PAIRS - 1) / (2 * LANES * PAIRS) * (2 * LANES * PAIRS);
+    if (n + threadIdx.x < end) sh.wide[n + threadIdx.x] = 0;
+    __syncthreads();
+    const u64x2* pairs = reinterpret_cast<const u64x2*>(sh.wide);
     for (uint32_t i = threadIdx.x / LANES; i < n; i += T / LANES) {
         const uint64_t mine = sh.wide[i];
         uint32_t above = 0;
-#pragma unroll 4
-        for (uint32_t j = part; j < n; j += LANES) above += sh.wide[j] > mine ? 1 : 0;
+        for (uint32_t j = part; j < end / 2; j += LANES * PAIRS) {
+            u64x2 v[PAIRS];
+#pragma unroll
+            for (uint32_t q = 0; q < PAIRS; ++q) v[q] = pairs[j + q * LANES];
+#pragma unroll
+            for (uint32_t q = 0; q < PAIRS; ++q) above += (v[q][0] > mine ? 1 : 0) + (v[q][1] > mine ? 1 : 0);
+        }
 #pragma unroll
         for (uint32_t d = 1; d < LANES; d *= 2) above += __shfl_xor(above, d);
         if (part == 0 && above < k) sh.best[above] = mine;
@@ -639,9 +691,20 @@ struct GradArgs {
 };
 
 // What the teacher takes from logit `id`: an id that the list holds twice loses the sum of both, in the list's order.
+// (One entry at a time its reads' latencies add up: 83 rows of 1731 with 128 entries 11.8 us, so 6.7.)
 __device__ inline float taken(const uint32_t* ids, const float* minus, uint32_t k, uint32_t id) {
     float v = 0.0f;
-    for (uint32_t i = 0; i < k; ++i) v += ids[i] == id ? minus[i] : 0.0f;
+    for (uint32_t i = 0; i < k; i += 16) {
+        u32x4 n[4];
+        f32x4 m[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            n[q] = reinterpret_cast<const u32x4*>(ids + i)[q];
+            m[q] = reinterpret_cast<const f32x4*>(minus + i)[q];
+        }
+#pragma unroll
+        for (int q = 0; q < 16; ++q) v += n[q / 4][q % 4] == id ? m[q / 4][q % 4] : 0.0f;
+    }
     return v;
 }
 
@@ -691,8 +754,9 @@ __global__ __launch_bounds__(GRAD_THREADS) void grad_rows(GradArgs a) {
             }
         }
     };
-    __shared__ uint32_t ids[TOP_MAX];
-    __shared__ float minus[TOP_MAX], own[TOP_MAX];
+    __shared__ __attribute__((aligned(16))) uint32_t ids[TOP_MAX];
+    __shared__ __attribute__((aligned(16))) float minus[TOP_MAX];
+    __shared__ float own[TOP_MAX];
     const uint32_t lo = seg * GRAD_SLOTS;
     if constexpr (MODE == TEACHER) {
         // The list's entries that lie in these slots: their probabilities, and their logits' own before any is overwritten.
@@ -754,8 +818,9 @@ __global__ __launch_bounds__(T) void distill_rows(GradArgs a) {
     constexpr int WAVES = T / 64;
     __shared__ double sums[WAVES];
     __shared__ float tops[WAVES];
-    __shared__ uint32_t ids[TOP_MAX];
-    __shared__ float minus[TOP_MAX], own[TOP_MAX];
+    __shared__ __attribute__((aligned(16))) uint32_t ids[TOP_MAX];
+    __shared__ __attribute__((aligned(16))) float minus[TOP_MAX];
+    __shared__ float own[TOP_MAX];
     __shared__ RowInfo shared_info;
     const uint32_t tid = threadIdx.x, lane = tid % 64, wave = tid / 64, row = a.row0 + blockIdx.x;
     const char* x = a.x + row * a.x_pitch * elem_size<DT>;
@@ -855,8 +920,10 @@ __global__ __launch_bounds__(T) void distill_rows(GradArgs a) {
 uint32_t ceil_div(uint64_t a, uint64_t b) { return static_cast<uint32_t>((a + b - 1) / b); }
 
 // Parts of a row, and slots to a part. Few rows are split until the chip has a workgroup for each compute unit, or two
-// while a part has over 64 KB, and each thread a slot; more only cost tickets (16 rows of 131072 in 256 parts 13.9 us, in
-// 512 15.9; 128 rows in 256 20.4, in 512 17.8). Where alternatives are wanted, no more slots than their maxima
+// while a part has over 64 KB, and each thread four slots; more only cost tickets (16 rows of 131072 in 256 parts 13.9 us, in
+// 512 15.9; 128 rows in 256 20.4, in 512 17.8). Rows that one workgroup reads in the time of a ticket and a join stay whole:
+// up to 2048 slots (20 rows of 16000 with 20 alternatives 7.8 us, in parts 10.3), more with more rows (150 of 32000: 10.5 us,
+// in two parts 13.3; 200 of 48000: 13.2 and 15.1). Where alternatives are wanted, no more slots than their maxima
 // have room for in LDS.
 struct Split {
     uint32_t segs, seg_slots;
@@ -866,7 +933,7 @@ Split split_rows(uint32_t rows, uint32_t cols, uint32_t size, uint32_t k) {
     const uint32_t slots = ceil_div(static_cast<uint64_t>(cols) + 7, 8) + 1, most = Shared<THREADS>::SLOT_BYTES / size;
     const uint32_t runs = static_cast<uint32_t>(static_cast<uint64_t>(cols) * size >> 16);
     uint32_t segs = std::max(ceil_div(256, rows), std::min(ceil_div(512, rows), runs));
-    segs = std::min(segs, ceil_div(slots, THREADS));
+    segs = slots <= (rows >= 128 ? 8192 : rows >= 16 ? 4096 : 2048) ? 1 : std::min(segs, ceil_div(slots, 4 * THREADS));
     if (k > 0) segs = std::max(std::min(segs, Shared<THREADS>::KEYS / k), ceil_div(slots, most));
     const uint32_t each = ceil_div(slots, segs);
     return {ceil_div(slots, each), each};
