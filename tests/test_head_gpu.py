@@ -310,6 +310,18 @@ def test_token_logprobs_of_equal_logits(hb, r, v, dtype):
 
 
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("v,k", [(600, 128), (1000, 128), (1999, 128), (500, 24), (16000, 128)])
+@pytest.mark.parametrize("r", [3, 130, 1100])
+def test_token_logprobs_of_rows_that_stay_candidates(hb, r, v, k, dtype):
+    """Fewer slots than alternatives, or most elements equal: nearly all of a row's elements are looked at."""
+    g = rng(950 + v)
+    x = g.standard_normal((r, v)) * 3
+    x[::3] = g.integers(0, 2, x[::3].shape)
+    x[1::3, v // 3:] = -5.0
+    check_logprobs(hb, H.to_bits(x, dtype), dtype, g.integers(0, v, r).astype(np.int32), k, 1.0)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
 def test_token_logprobs_of_a_peak(hb, dtype):
     """Almost all of the probability on one logit: the small entropy keeps its digits."""
     g = rng(1000)
