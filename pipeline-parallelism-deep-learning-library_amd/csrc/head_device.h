@@ -153,6 +153,17 @@ __device__ inline double wave_sum(double v) {
     return __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
 }
 
+__device__ inline uint32_t wave_sum(uint32_t u) {
+    int v = static_cast<int>(u);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);
+    return static_cast<uint32_t>(__builtin_amdgcn_readlane(v, 63));
+}
+
 inline void launched(Context* ctx, const char* name) {
     check_hip(hipGetLastError(), name);
     note_launch(ctx, name);

@@ -137,6 +137,7 @@ struct Shared {
     static constexpr uint32_t SLOT_BYTES = T == 64 ? 4096 : 16384;  // of the slots' maxima: 2 or 4 bytes each
     static constexpr uint32_t KEYS = SLOT_BYTES / 8;                // which take the maxima's place
     static constexpr uint32_t LIST = T == 64 ? 64 : 512;            // slots whose elements are looked at
+    static constexpr uint32_t COUNTS = 96;                          // three for each two bits of a key
     alignas(16) uint64_t wide[KEYS];
     uint64_t best[TOP_MAX];
     float tops[T];
@@ -144,7 +145,7 @@ struct Shared {
     double s[WAVES], u[WAVES];
     float m[WAVES];
     float bound;  // below the k-th largest
-    uint32_t listed, found, count, counts[24];
+    uint32_t listed, found, counts[COUNTS];
     bool last;
 };
 
@@ -182,31 +183,46 @@ __device__ inline float threshold(const float* tops, uint32_t k) {
 template <int T>
 __device__ inline uint32_t total(Shared<T>& sh, uint32_t mine) {
     __syncthreads();
-    if (threadIdx.x == 0) sh.count = 0;
+    if (threadIdx.x == 0) sh.counts[0] = 0;
     __syncthreads();
-    if (mine) atomicAdd(&sh.count, mine);
+    mine = wave_sum(mine);
+    if (threadIdx.x % 64 == 0) atomicAdd(&sh.counts[0], mine);
     __syncthreads();
-    return sh.count;
+    return sh.counts[0];
 }
 
-// The k-th largest of n keys that differ from one another, or 0 where there are fewer, bit by bit.
+// The largest number that at least k of n keys reach, told from bit `bits` - 1 down to bit `end`, two bits at a time (both
+// even); `t` has the bits above. With k keys that differ from one another and all bits, the k-th largest key.
 template <int T, typename F>
-__device__ inline uint64_t kth_key(Shared<T>& sh, uint32_t n, uint32_t k, F&& key) {
-    uint64_t bound = 0;
-    for (uint64_t bit = 1ull << 63; bit != 0; bit >>= 1) {
-        uint32_t c = 0;
-        for (uint32_t i = threadIdx.x; i < n; i += T) c += key(i) >= (bound | bit) ? 1 : 0;
-        if (total(sh, c) >= k) bound |= bit;
-    }
+__device__ uint64_t kth_key(Shared<T>& sh, uint64_t t, uint32_t bits, uint32_t end, uint32_t n, uint32_t k, F&& key) {
     __syncthreads();
-    return bound;
+    for (uint32_t i = threadIdx.x; i < Shared<T>::COUNTS; i += T) sh.counts[i] = 0;
+    __syncthreads();
+    uint32_t* count = sh.counts;
+    for (uint32_t shift = bits; shift != end; count += 3) {
+        shift -= 2;
+        uint32_t c[3] = {0, 0, 0};
+        for (uint32_t i = threadIdx.x; i < n; i += T) {
+            const uint64_t v = key(i);
+#pragma unroll
+            for (uint64_t q = 0; q < 3; ++q) c[q] += v >= (t | (q + 1) << shift) ? 1 : 0;
+        }
+#pragma unroll
+        for (int q = 0; q < 3; ++q) {
+            c[q] = wave_sum(c[q]);
+            if (threadIdx.x % 64 == 0) atomicAdd(&count[q], c[q]);
+        }
+        __syncthreads();
+        t |= (count[2] >= k ? 3ull : count[1] >= k ? 2ull : count[0] >= k ? 1ull : 0ull) << shift;
+    }
+    return t;
 }
 
 // Keeps of the n keys in sh.wide those that can be among the k largest, told by the first sixteen bits, or where equal
 // ones are too many by all; returns how many.
 template <int T>
 __device__ uint32_t narrow(Shared<T>& sh, uint32_t n, uint32_t k) {
-    constexpr uint32_t HELD = Shared<T>::KEYS / T, STEPS = 8;
+    constexpr uint32_t HELD = Shared<T>::KEYS / T;
     uint64_t held[HELD];
 #pragma unroll
     for (uint32_t i = 0; i < HELD; ++i) held[i] = i * T + threadIdx.x < n ? sh.wide[i * T + threadIdx.x] : 0;
@@ -221,26 +237,10 @@ __device__ uint32_t narrow(Shared<T>& sh, uint32_t n, uint32_t k) {
         __syncthreads();
         return sh.found;
     };
-    if (threadIdx.x < 3 * STEPS) sh.counts[threadIdx.x] = 0;
-    __syncthreads();
-    uint64_t t = 0;
-    for (uint32_t step = 0; step < STEPS; ++step) {
-        const uint32_t shift = 62 - 2 * step;
-#pragma unroll
-        for (uint64_t c = 0; c < 3; ++c) {
-            uint32_t above = 0;
-#pragma unroll
-            for (uint32_t i = 0; i < HELD; ++i) above += __popcll(__ballot(held[i] >= (t | (c + 1) << shift)));
-            if (threadIdx.x % 64 == 0) atomicAdd(&sh.counts[3 * step + c], above);
-        }
-        __syncthreads();
-        const uint32_t* count = sh.counts + 3 * step;
-        t |= (count[2] >= k ? 3ull : count[1] >= k ? 2ull : count[0] >= k ? 1ull : 0ull) << shift;
-    }
+    auto key = [&](uint32_t i) { return sh.wide[i]; };
+    const uint64_t t = kth_key(sh, 0, 64, 48, n, k, key);
     n = keep(t);
-    if (n <= 2 * T) return n;
-    const uint64_t bound = kth_key(sh, n, k, [&](uint32_t i) { return sh.wide[i]; });
-    return keep(bound);
+    return n <= 2 * T ? n : keep(kth_key(sh, t, 48, 0, n, k, key));
 }
 
 // sh.best, zeros so far, = the k largest of the n keys in sh.wide, in order: each key goes to the place that as
@@ -306,9 +306,14 @@ __device__ void top_of_slots(Shared<T>& sh, const Slots<DT>& row, uint32_t lo, u
         many = total(sh, c) > Shared<T>::KEYS;
     }
     if (many) {
-        auto slot = [&](uint32_t i) { return key_of(Max::unpack(maxima[i]), i); };
-        const uint64_t bound = kth_key(sh, n, k, slot);
-        t = key_value(bound);
+        // A slot's maximum, without the bits that its type leaves zero, above the slot's number.
+        constexpr uint32_t DROPPED = DT == LG_DTYPE_F32 ? 0 : DT == LG_DTYPE_BF16 ? 16 : 12, NUMBER = 14;
+        static_assert(Shared<T>::SLOT_BYTES / elem_size<DT> <= 1u << NUMBER, "slots have their numbers");
+        auto slot = [&](uint32_t i) {
+            return static_cast<uint64_t>(order(Max::unpack(maxima[i])) >> DROPPED) << NUMBER | ((1u << NUMBER) - 1 - i);
+        };
+        const uint64_t bound = kth_key(sh, 0, 32 - DROPPED + NUMBER, 0, n, k, slot);
+        t = unorder(static_cast<uint32_t>(bound >> NUMBER) << DROPPED);
         if (tid == 0) sh.listed = 0;
         __syncthreads();
         for (uint32_t i = tid; i < n; i += T) {
@@ -534,7 +539,7 @@ __device__ Part join_parts(const PassArgs& a, Shared<T>& sh, uint32_t at) {
         }
         __syncthreads();
         if (sh.found > Shared<T>::KEYS) {  // many equal ones
-            const uint64_t bound = kth_key(sh, all, k, key);
+            const uint64_t bound = kth_key(sh, 0, 64, 0, all, k, key);
             if (tid == 0) sh.found = 0;
             __syncthreads();
             for (uint32_t i = tid; i < all; i += T) {

@@ -322,6 +322,17 @@ def test_token_logprobs_of_rows_that_stay_candidates(hb, r, v, k, dtype):
 
 
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("r,v", [(2, 9000), (3, 70000), (1100, 4000)])
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+def test_token_logprobs_of_logits_a_unit_apart(hb, sign, r, v, dtype):
+    """Eight neighbouring numbers of the type, so that what tells the alternatives is the last bits and the ids."""
+    g = rng(970 + v)
+    x = sign * (1.0 + g.integers(0, 8, (r, v)) * 2.0 ** {F32: -23, F16: -10, BF16: -7}[dtype])
+    for k in (5, 24, 128):
+        check_logprobs(hb, H.to_bits(x, dtype), dtype, g.integers(0, v, r).astype(np.int32), k, 1.0)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
 def test_token_logprobs_of_a_peak(hb, dtype):
     """Almost all of the probability on one logit: the small entropy keeps its digits."""
     g = rng(1000)
