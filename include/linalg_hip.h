@@ -362,7 +362,8 @@ lg_core_error lg_backend_upload_into(lg_ctx* ctx, void* stream, const uint8_t* b
  * whose bytes intersect another operand's LG_CORE_ALIAS), on any error nothing is launched or
  * written, and calls enqueue on `stream` (NULL = context stream) and return before the device
  * finishes. Matrices have rows of unit stride at any pitch of at least their length and at any
- * offset (a window of a larger matrix); vectors have unit stride. Extents are below 2^31 - 256.
+ * offset (a window of a larger matrix); vectors have unit stride. Extents are below 2^31 - 256,
+ * quantize_blocks' columns and the logits of rows whose alternatives are wanted at most 2^29.
  * Rows that are split over workgroups, and distill_grad, use the context's shared scratch: under
  * stream capture see "Split scratch" above. Results do not depend on the order in which
  * workgroups run.

@@ -20,6 +20,7 @@ namespace lg {
 namespace {
 
 constexpr uint64_t EXTENT_MAX = 0x7fffff00ull;  // a tile's last row or slot still fits 32 bits
+constexpr uint64_t ROW_MAX = 1ull << 29;        // columns of a row whose tiles one launch, or whose parts the scratch, has to hold
 
 uint32_t element_bytes(const lg_tensor* t) {
     switch (t->dtype) {
@@ -127,10 +128,10 @@ void storage(Operand& o) {
     }
     if (o.t->base == nullptr) core_fail(LG_CORE_SHAPE, std::string(o.name) + " has no storage");
     if (o.t->offset > o.t->bytes || (lines > 1 && o.pitch > o.t->bytes / (lines - 1))) core_fail(LG_CORE_SHAPE, past);
-    const uint64_t elements = o.t->offset + (lines - 1) * o.pitch + length;  // below 3 * 2^64 / size only if bytes are
-    if (o.t->offset > UINT64_MAX / 4 || (lines - 1) * o.pitch > UINT64_MAX / 4 || elements > o.t->bytes / size) {
-        core_fail(LG_CORE_SHAPE, past);
-    }
+    // Both terms are at most `bytes` here; their sum and the length cannot wrap once they are below a quarter of all.
+    if (o.t->offset > UINT64_MAX / 4 || (lines - 1) * o.pitch > UINT64_MAX / 4) core_fail(LG_CORE_SHAPE, past);
+    const uint64_t elements = o.t->offset + (lines - 1) * o.pitch + length;
+    if (elements > o.t->bytes / size) core_fail(LG_CORE_SHAPE, past);
     o.first = base + o.t->offset * size;
     o.end = base + elements * size;
     if (o.first % size != 0) core_fail(LG_CORE_UNSUPPORTED_LAYOUT, std::string(o.name) + " is misaligned for its element type");
@@ -204,6 +205,7 @@ lg_core_error lg_backend_quantize_blocks(lg_ctx* ctx, void* stream, const lg_ten
         need(ox.rows == oq.rows && ox.cols == oq.cols, "quantize_blocks needs x and q of one shape");
         QuantizeArgs a{};
         a.block = scale_block(os, oq.rows, oq.cols);
+        need(oq.cols <= ROW_MAX, "quantize_blocks takes rows of at most 2^29 columns");
         dtype(ox, {LG_DTYPE_F32, LG_DTYPE_F16, LG_DTYPE_BF16});
         dtype(oq, {LG_DTYPE_E4M3});
         dtype(os, {LG_DTYPE_F32, LG_DTYPE_E8M0});
@@ -303,6 +305,7 @@ lg_core_error lg_backend_token_logprobs(lg_ctx* ctx, void* stream, const lg_tens
         need(!st || (st.rows == x.rows && st.cols == 2), "stats needs shape [rows, 2]");
         need(!top || (top.rows == x.rows && ids.rows == x.rows && top.cols == ids.cols && top.cols <= TOP_MAX),
              "top_logprobs and top_ids need shape [rows, k] with k of at most 128");
+        need(!top || top.cols == 0 || x.cols <= ROW_MAX, "alternatives are of rows of at most 2^29 logits");
         check_temperature(temperature);
         dtype(x, {LG_DTYPE_F32, LG_DTYPE_F16, LG_DTYPE_BF16});
         for (const Operand* o : {&t, &ids}) dtype(*o, {LG_DTYPE_I32});

@@ -572,7 +572,8 @@ struct Piece {
 // A pass over a part of a row; the row's last workgroup finishes it. Bound by reading the logits, and by the latency of
 // what follows a row's last slot, under which other rows' workgroups of the compute unit read: 4096 rows of 32768 bf16
 // 44 us without entropy and alternatives (6.0 TB/s), 51 us with entropy, 59 and 65 us with 20 and 64 alternatives (by
-// workgroups of eight waves 57, 67 and 73 us); one row of 131072 with 20 alternatives 10.4 us.
+// workgroups of eight waves 57, 67 and 73 us); one row of 131072 with 20 alternatives 10.2 us, 48 rows of 100003 f32 with a
+// teacher 10 us.
 template <uint32_t DT, bool ENTROPY, bool TOP, bool DISTILL, int T>
 __global__ __launch_bounds__(T) void row_pass(PassArgs a) {
     __shared__ Shared<T> sh;
@@ -716,7 +717,8 @@ __device__ inline float taken(const uint32_t* ids, const float* minus, uint32_t 
 enum GradMode { LOGPROB, LOGPROB_ENTROPY, TEACHER };
 
 // dx of GRAD_SLOTS slots of a row: an element at a time from the row's statistics. The token's own term
-// joins in its slot; a teacher's are written over the dense gradient when it is complete, from logits read before.
+// joins in its slot; a teacher's are written over the dense gradient when it is complete, from logits read before. Bound by
+// memory: 1024 rows of 50001 f32 83.5 us (4.9 TB/s).
 template <uint32_t DT, GradMode MODE>
 __global__ __launch_bounds__(GRAD_THREADS) void grad_rows(GradArgs a) {
     const uint32_t tid = threadIdx.x, at = blockIdx.x / a.segs, seg = blockIdx.x % a.segs, row = a.row0 + at;
@@ -816,8 +818,8 @@ __global__ __launch_bounds__(GRAD_THREADS) void grad_rows(GradArgs a) {
 
 // Loss and gradient of whole rows, a workgroup each: the row stays in registers, NV slots a thread, from its one read
 // to its gradient's one write. The first wave works out the teacher's list beside the sums. Bound by memory where
-// at least two rows share a compute unit: 4096 rows of 65536 bf16 226 us (4.75 TB/s read and written), in two passes
-// 306 us, with eight slots a thread and one row a compute unit 304 us; of 65536 f32 429 us (5.0 TB/s), in two passes 576 us.
+// at least two rows share a compute unit: 4096 rows of 65536 bf16 210 us (5.1 TB/s read and written, a large copy's rate), in
+// two passes 306 us, with eight slots a thread and one row a compute unit 304 us.
 template <uint32_t DT, int T, int NV>
 __global__ __launch_bounds__(T) void distill_rows(GradArgs a) {
     constexpr int WAVES = T / 64;
@@ -957,11 +959,11 @@ void launch_pass(lg_ctx* ctx, hipStream_t s, const PassArgs& a, uint32_t rows) {
     launched(ctx, DISTILL ? "row_pass_distill" : TOP ? "row_pass_top" : "row_pass");
 }
 
-// Rows in batches of `most`, and of no more than a launch's threads have 32-bit numbers for.
+// Rows in batches of `most`, and of no more than a launch's threads have 32-bit numbers for; the longest rows' parts are
+// 2^18 workgroups, and fill 17 MB of scratch with their alternatives.
 template <typename F>
 void batches(uint32_t rows, uint64_t wgs_per_row, uint64_t most, F&& launch) {
     const uint64_t batch = std::min<uint64_t>(most, (1ull << 22) / wgs_per_row);
-    if (batch == 0) fail_invalid("rows of so many logits do not fit a launch or its scratch");
     for (uint64_t r = 0; r < rows; r += batch) launch(static_cast<uint32_t>(r), static_cast<uint32_t>(std::min<uint64_t>(batch, rows - r)));
 }
 

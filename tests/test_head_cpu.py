@@ -36,6 +36,15 @@ def changed(args, i, t):
     return out
 
 
+def test_rows_of_more_columns_than_a_launch_holds():
+    for cols, want in ((1 << 29, PASSED), ((1 << 29) + 1, "Shape")):
+        wide = [tensor(BF16, [1, cols]), tensor(E4M3, [1, cols]), tensor(F32, [1, -(-cols // 128)])]
+        assert kind("quantize_blocks", *wide) == want
+        outs = [tensor(F32, [1, 5]), tensor(I32, [1, 5])]
+        assert kind("token_logprobs", wide[0], None, 1.0, None, None, None, *outs) == want
+        assert kind("token_logprobs", wide[0], None, 1.0, None, tensor(F32, [1]), None, None, None) == PASSED
+
+
 def test_quantize_blocks_refusals():
     x, q, s = tensor(BF16, [300, 500]), tensor(E4M3, [300, 500]), tensor(F32, [300, 4])
     ok = [x, q, s]
