@@ -13,8 +13,6 @@
 // conversion, or are the fp8 instruction's own operands.
 #pragma once
 
-#include <algorithm>
-
 #include "head_device.h"
 
 namespace lg {
@@ -590,8 +588,9 @@ inline Plan plan_of(const GemmBlocksArgs& g, bool direct) {
     if (g.a_pitch >= (1 << 23) || g.b_pitch >= (1 << 23)) return THIN;
     // The fp8 instruction's precision is enough for 16-bit outputs of long sums.
     const bool fast = g.out != LG_DTYPE_F32 && g.k >= 512;
-    // Operands beyond the caches arrive at 6 TB/s for every kernel, soonest for the first.
-    const uint64_t reading = (static_cast<uint64_t>(g.m) + g.n) * g.k / 60000;
+    // What B's bytes take at 6 TB/s: a kernel that the model has below it waits for memory, for which THIN waits least
+    // (1x65536x4096 39 us, on 32x64 fp8 tiles 53 us).
+    const uint64_t reading = static_cast<uint64_t>(g.n) * g.k / 60000;
     uint64_t best = ~0ull;
     Plan plan = THIN;
     for (int p = THIN; p < (fast ? PLANS : FP8_256); ++p) {
@@ -600,9 +599,9 @@ inline Plan plan_of(const GemmBlocksArgs& g, bool direct) {
         const auto& t = direct ? c.direct : c.any;
         const uint64_t tiles = static_cast<uint64_t>((g.m + c.m - 1) / c.m) * ((g.n + c.n - 1) / c.n);
         const uint64_t turns = ((g.k + BLOCK_K - 1) / BLOCK_K + c.groups - 1) / c.groups;
-        uint64_t time = c.share == 1 || tiles <= 256 ? (tiles + 255) / 256 * (t.fixed + t.turn * turns)
-                                                     : (tiles + 256 * c.share - 1) / (256 * c.share) * (t.shared_fixed + t.shared_turn * turns);
-        time = std::max(time, reading);
+        const uint64_t time = c.share == 1 || tiles <= 256 ? (tiles + 255) / 256 * (t.fixed + t.turn * turns)
+                                                           : (tiles + 256 * c.share - 1) / (256 * c.share) * (t.shared_fixed + t.shared_turn * turns);
+        if (p == THIN && time <= reading) return THIN;
         if (time < best) {
             best = time;
             plan = static_cast<Plan>(p);
