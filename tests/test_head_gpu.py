@@ -62,6 +62,21 @@ def test_quantize_blocks_bit_for_bit(hb, shape, pad, dtype, block, scales, trans
     assert np.array_equal(q.read(), want_q)
 
 
+@pytest.mark.parametrize("transposed", [False, True])
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("shape", [(256, 1024), (128, 128), (1000, 640), (1150, 2304), (2000, 64)])
+def test_quantize_blocks_of_whole_lines(hb, shape, dtype, transposed):
+    """Operands of their own, whose rows are whole lines of memory or nearly."""
+    g = rng(150 + shape[0])
+    r, c = shape
+    bits = matrix(g, c, r, dtype) if transposed else matrix(g, r, c, dtype)
+    for block in (1, 128):
+        x, q, s = Window(hb, dtype, bits), Window(hb, E4M3, shape=shape), Window(hb, E8M0, shape=B.scales_shape(shape, block))
+        hb.quantize_blocks(B.transpose_matrix(x.t) if transposed else x.t, q.t, s.t)
+        want_q, want_s = H.quantize(H.values(bits.T if transposed else bits, dtype).astype(np.float32), block, E8M0)
+        assert np.array_equal(s.read(), want_s) and np.array_equal(q.read(), want_q)
+
+
 @pytest.mark.parametrize("scales", [F32, E8M0])
 @pytest.mark.parametrize("block", [1, 128])
 def test_quantize_blocks_at_the_ends_of_the_range(hb, block, scales):
