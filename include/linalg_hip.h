@@ -392,8 +392,9 @@ lg_core_error lg_backend_quantize_blocks(lg_ctx* ctx, void* stream, const lg_ten
  * F32, F16 or BF16. The sums are f32, in a fixed order of the plan's own: of exact products, but into
  * F16 or BF16 from K = 512 on of products in groups of eight along K, each kept to 2^-13 of its
  * group's largest (what the fp8 matrix instructions keep: 1.5e-5 of the norm for normal
- * operands). alpha * sum and beta * c add in f32 and round once to c's type. An element times its
- * E8M0 scale counts as zero below 2^-126 and as infinite from 2^128. beta = 0 does not read c;
+ * operands). alpha * sum and beta * c add in f32 and round once to c's type. Two F32 scales are
+ * multiplied with each other first, in f32; an element times its E8M0 scale counts as zero below
+ * 2^-126 and as infinite from 2^128. beta = 0 does not read c;
  * alpha = 0 reads neither a nor b. */
 lg_core_error lg_backend_gemm_blocks(lg_ctx* ctx, void* stream, const lg_tensor* a,
                                      const lg_tensor* a_scales, const lg_tensor* b,
