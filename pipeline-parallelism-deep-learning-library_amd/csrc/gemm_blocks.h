@@ -13,6 +13,8 @@
 // conversion, or are the fp8 instruction's own operands.
 #pragma once
 
+#include <algorithm>
+
 #include "head_device.h"
 
 namespace lg {
@@ -562,7 +564,7 @@ bool copies_fit(const GemmBlocksArgs& g) {
 // part and one for every turn of its groups along K. The figures, in hundredths of a microsecond, are a fit over 320
 // products with sizes spread evenly over the logarithms of 1 to 8192 rows, 128 to 16384 columns and K of 200 to 8192, each
 // timed on every kernel: the kernel with the least modelled time took 1.04 times the time of the fastest on
-// average. `share`: workgroups that share a compute unit, from 257 tiles on.
+// average. `share`: workgroups that share a compute unit, from 257 tiles on; 0: many, without rounds.
 struct Cost {
     uint32_t m, n, groups, share;
     struct {
@@ -571,7 +573,7 @@ struct Cost {
 };
 enum Plan { THIN, BF16_128, BF16_64, BF16_32X64, BF16_32, BF16_16, FP8_256, FP8_128, FP8_64, FP8_32X64, FP8_32, PLANS };
 constexpr Cost COSTS[PLANS] = {
-    {16, 32, 4, 3, {76, 142, 0, 361}, {71, 55, 29, 135}},
+    {16, 32, 4, 0, {76, 142, 0, 120}, {71, 55, 15, 50}},
     {128, 128, 1, 2, {246, 133, 309, 314}, {177, 115, 314, 192}},
     {64, 64, 2, 2, {134, 128, 270, 187}, {75, 88, 152, 145}},
     {32, 64, 4, 1, {138, 157, 0, 0}, {107, 105, 0, 0}},
@@ -588,26 +590,27 @@ inline Plan plan_of(const GemmBlocksArgs& g, bool direct) {
     if (g.a_pitch >= (1 << 23) || g.b_pitch >= (1 << 23)) return THIN;
     // The fp8 instruction's precision is enough for 16-bit outputs of long sums.
     const bool fast = g.out != LG_DTYPE_F32 && g.k >= 512;
-    // What B's bytes take at 6 TB/s: a kernel that the model has below it waits for memory, for which THIN waits least
-    // (1x65536x4096 39 us, on 32x64 fp8 tiles 53 us).
-    const uint64_t reading = static_cast<uint64_t>(g.n) * g.k / 60000;
-    uint64_t best = ~0ull;
-    Plan plan = THIN;
-    for (int p = THIN; p < (fast ? PLANS : FP8_256); ++p) {
-        if (p == THIN ? g.m > 16 : p == FP8_256 && !direct) continue;
+    auto time = [&](int p) {
         const Cost& c = COSTS[p];
         const auto& t = direct ? c.direct : c.any;
         const uint64_t tiles = static_cast<uint64_t>((g.m + c.m - 1) / c.m) * ((g.n + c.n - 1) / c.n);
         const uint64_t turns = ((g.k + BLOCK_K - 1) / BLOCK_K + c.groups - 1) / c.groups;
-        const uint64_t time = c.share == 1 || tiles <= 256 ? (tiles + 255) / 256 * (t.fixed + t.turn * turns)
-                                                           : (tiles + 256 * c.share - 1) / (256 * c.share) * (t.shared_fixed + t.shared_turn * turns);
-        if (p == THIN && time <= reading) return THIN;
-        if (time < best) {
-            best = time;
+        if (c.share == 0 && tiles > 256) return tiles * (t.shared_fixed + t.shared_turn * turns) / 256;
+        return c.share <= 1 || tiles <= 256 ? (tiles + 255) / 256 * (t.fixed + t.turn * turns)
+                                              : (tiles + 256 * c.share - 1) / (256 * c.share) * (t.shared_fixed + t.shared_turn * turns);
+    };
+    Plan plan = BF16_128;
+    uint64_t best = time(plan);
+    for (int p = BF16_64; p < (fast ? PLANS : FP8_256); ++p) {
+        if (p == FP8_256 && !direct) continue;
+        if (const uint64_t t = time(p); t < best) {
+            best = t;
             plan = static_cast<Plan>(p);
         }
     }
-    return plan;
+    // Tiles read B at 4.8 TB/s at the best (1x65536x4096 53 us, THIN 39 us; 1x32000x2048 16.7 and 13.2 us).
+    const uint64_t reading = static_cast<uint64_t>(g.n) * g.k / 48000;
+    return g.m <= 16 && time(THIN) <= std::max(best, reading) ? THIN : plan;
 }
 
 template <uint32_t OUT, bool DIRECT, bool E8M0, bool BROWS>

@@ -169,7 +169,7 @@ PLANS = [
     (9, 600, 128, F32, "thin"), (5, 70, 100, BF16, "thin"), (40, 1024, 1024, F32, "bf16_16x16"), (3, 1000, 700, F32, "bf16_16x16_any"),
     (33, 1000, 301, F32, "bf16_16x16_any"), (60, 2201, 1040, F32, "bf16_32x32"), (3, 5000, 530, F32, "bf16_32x32_any"),
     (257, 1000, 1040, F32, "bf16_32x64"), (2074, 17, 257, BF16, "bf16_32x64_any"), (90, 3000, 530, F32, "bf16_32x64_any"),
-    (16, 8200, 256, BF16, "bf16_64x64"), (1024, 1024, 256, F32, "bf16_64x64"), (300, 900, 200, F32, "bf16_64x64_any"),
+    (16, 8200, 256, BF16, "thin"), (1024, 1024, 256, F32, "bf16_64x64"), (300, 900, 200, F32, "bf16_64x64_any"),
     (2048, 2560, 272, F32, "bf16_128x128"), (1030, 1001, 127, F32, "bf16_128x128_any"), (2049, 2561, 201, F16, "bf16_128x128_any"),
     (60, 2201, 1040, F16, "fp8_32x32"), (40, 1501, 1041, F16, "fp8_32x32_any"), (130, 2100, 1040, BF16, "fp8_32x64"),
     (65, 4099, 1300, F16, "fp8_32x64_any"), (1024, 2048, 528, BF16, "fp8_64x64"), (500, 1030, 530, BF16, "fp8_64x64_any"),
