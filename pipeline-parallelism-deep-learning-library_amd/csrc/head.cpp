@@ -165,15 +165,15 @@ void check_temperature(float t) {
 
 uint32_t u32(uint64_t v) { return static_cast<uint32_t>(v); }
 
-// In parts whose tiles a launch has numbers for, whole blocks of 128 rows each.
+// In parts whose threads a launch has 32-bit numbers for, whole blocks of 128 rows each. (Pitches from 2^23 on take small tiles.)
 void launch_gemm_blocks(lg_ctx* ctx, hipStream_t s, const GemmBlocksArgs& g) {
-    constexpr uint32_t PART = 1u << 22;
+    const uint32_t part = std::max(g.a_pitch, g.b_pitch) >= 1 << 23 ? 1u << 16 : 1u << 22;
     const uint64_t scale = g.e8m0 ? 1 : 4, out = g.out == LG_DTYPE_F32 ? 4 : 2;
-    for (uint32_t m = 0; m < g.m; m += PART) {
-        for (uint32_t n = 0; n < g.n; n += PART) {
+    for (uint32_t m = 0; m < g.m; m += part) {
+        for (uint32_t n = 0; n < g.n; n += part) {
             GemmBlocksArgs p = g;
-            p.m = std::min(g.m - m, PART);
-            p.n = std::min(g.n - n, PART);
+            p.m = std::min(g.m - m, part);
+            p.n = std::min(g.n - n, part);
             p.a += m * g.a_pitch;
             p.b += n * g.b_pitch;
             p.sa = static_cast<const char*>(g.sa) + m / g.a_block * g.sa_pitch * scale;

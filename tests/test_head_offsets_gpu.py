@@ -75,3 +75,17 @@ def test_blocks_far_apart(hb):
     hb.gemm_blocks(qa.t, sa.t, B.transpose_matrix(qb.t), sb.t, c.t)
     va, vb = H.unquantized(wa, wsa, 1, F32), H.unquantized(wb, wsb, 128, F32)
     close(c.read(), va @ vb.T, 140 * 2.0 ** -24 * (np.abs(va) @ np.abs(vb).T), 1e-7, "c")
+
+
+def test_columns_beyond_one_launch(hb):
+    """A's rows far apart, and more rows of B than one launch takes then."""
+    g = rng(2300)
+    n, k = (1 << 16) + 300, 130
+    a, b = g.standard_normal((3, k)).astype(np.float32), g.standard_normal((n, k)).astype(np.float32)
+    for block in (1, 128):
+        wa, wsa = H.quantize(a, 1, F32)
+        wb, wsb = H.quantize(b, block, F32)
+        qa, qb, c = Spread(hb, E4M3, wa), Window(hb, E4M3, wb), Window(hb, F32, shape=[3, n], pad=1)
+        hb.gemm_blocks(qa.t, Window(hb, F32, wsa).t, B.transpose_matrix(qb.t), Window(hb, F32, wsb).t, c.t)
+        va, vb = H.unquantized(wa, wsa, 1, F32), H.unquantized(wb, wsb, block, F32)
+        close(c.read(), va @ vb.T, 140 * 2.0 ** -24 * (np.abs(va) @ np.abs(vb).T), 1e-7, "c")
