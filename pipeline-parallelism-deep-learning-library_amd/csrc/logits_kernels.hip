@@ -244,10 +244,11 @@ __device__ uint32_t narrow(Shared<T>& sh, uint32_t n, uint32_t k) {
 }
 
 // sh.best, zeros so far, = the k largest of the n keys in sh.wide, in order: each key goes to the place that as
-// many others exceed it, counted by four lanes, sixteen pairs at a time. Keys differ from one another.
+// many others exceed it, counted by two lanes, eight pairs each at a time (60 rows of 1505, 64
+// alternatives: 7.3 us, by one lane 7.6, by four 7.6, by eight 7.8). Keys differ from one another.
 template <int T>
 __device__ inline void rank_keys(Shared<T>& sh, uint32_t n, uint32_t k) {
-    constexpr uint32_t LANES = 4, PAIRS = 8;
+    constexpr uint32_t LANES = 2, PAIRS = 8;
     if (n > 2 * T) n = narrow(sh, n, k);  // a row of 1000 with 128 alternatives, all of them keys, 13 us; by ranks alone 48
     const uint32_t part = threadIdx.x % LANES, end = (n + 2 * LANES * PAIRS - 1) / (2 * LANES * PAIRS) * (2 * LANES * PAIRS);
     if (n + threadIdx.x < end) sh.wide[n + threadIdx.x] = 0;
@@ -571,8 +572,8 @@ struct Piece {
 
 // A pass over a part of a row; the row's last workgroup finishes it. Bound by reading the logits, and by the latency of
 // what follows a row's last slot, under which other rows' workgroups of the compute unit read: 4096 rows of 32768 bf16
-// 44 us without entropy and alternatives (6.0 TB/s), 51 us with entropy, 59 and 65 us with 20 and 64 alternatives (by
-// workgroups of eight waves 57, 67 and 73 us); one row of 131072 with 20 alternatives 10.2 us, 48 rows of 100003 f32 with a
+// 44 us without entropy and alternatives (6.0 TB/s), 51 us with entropy, 58 and 64 us with 20 and 64 alternatives (by
+// workgroups of eight waves 57, 67 and 73 us); one row of 131072 with 20 alternatives 10.1 us, 48 rows of 100003 f32 with a
 // teacher 10 us.
 template <uint32_t DT, bool ENTROPY, bool TOP, bool DISTILL, int T>
 __global__ __launch_bounds__(T) void row_pass(PassArgs a) {
